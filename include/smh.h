@@ -494,6 +494,57 @@ int smh_decode_stack_of(const smh_layer *const *layers, int n_layers, smh_pass *
                         smh_stream_t stream);
 int smh_decode_finish(const smh_layer *last, smh_pass *pass, const void *norm_weight, float eps, void *out, smh_stream_t stream);
 
+/* ---- paged 8-bit cache -----------------------------------------------------------------------------------------------
+ * K and V of several sequences of any length, in 8 bits.  A block is 64 consecutive rows of a sequence; for each kv head a whole block holds codes
+ * u = rint(x * 127 / amax) + 128 and the scale amax / 127 of K and of V: x is read as (u - 128) * scale.  The open block - the last one, while it has fewer than
+ * 64 rows - is held in fp16 and becomes codes when its 64th row arrives, so every row is quantised once and the cache does not depend on
+ * how the rows came in.  No counterpart in the reference, whose caches are fp16 and Q4_0 (hf_model_q40_kv_shared.py:252-409).
+ *   codes_k       uint8 [n_pages, Hkv, 64, 128]
+ *   codes_v       uint8 [n_pages, Hkv, 128, 64]: place 16 g + 8 u + 4 j + i of a line is row 32 u + 16 j + 4 g + i of the block (g, i < 4; u, j < 2)
+ *   scales        fp32 [n_pages, Hkv, 2]: of K, of V
+ *   open_k        fp16 [B, Hkv, 64, 128]; open_v fp16 [B, Hkv, 128, 64] in the order of codes_v
+ *   pages         int32 [B, pages_stride], pages_cols in use: block j of sequence b is page pages[b, j].  Read ids are cut to 0 .. n_pages - 1; a block whose id
+ *                 is outside, or past pages_cols, is not written
+ *   lens          int32 [B] on the device: rows of each sequence before the call (the call does not change them).  A sequence has at most
+ *                 pages_cols * 64 + 63 rows; what lies past that is neither read nor written
+ *   cu            NULL: one new row for each sequence (T = B).  Else int32 [B + 1] on the device: the new rows of sequence b are rows cu[b] .. cu[b + 1] - 1 of
+ *                 q, k, v (none is fine), of which the first max_new count.  Rows of no sequence are left as they are in the outputs.
+ * A row of k or v with an infinity or a NaN makes its block's values of that head NaN (for an open block: those of that row, and the outputs of queries that
+ * see any row of the block).  D is 128.  Tensors are 16-byte aligned (scales 8); *_stride is the distance of two tokens in values, a multiple of 8, heads are contiguous.
+ *
+ * smh_kv8_append   rotates q and k (apply_rotary_emb, hf_model_q40_kv_shared.py:173-203, by the fp16 tables [table_rows, 64] at the row's place in its
+ *                  sequence, cut to the last table row; fp32 sums of exact products, one rounding to fp16), writes q to q_out [T, H, 128] and k, v into the cache.
+ * smh_kv8_attn     attention of the new rows over the cache that smh_kv8_append left: the query of place i sees rows j <= i, with a window > 0 only
+ *                  those with j > i - window or j < sinks.  out [T, H, 128] fp16; any H / Hkv.  max_len: an upper bound of lens[b] + new rows; it decides how the work is
+ *                  split, not what is read.  workspace: smh_kv8_attn_workspace_bytes(...) bytes, any contents; calls that overlap in time need one each.
+ * smh_kv8_rows     rows first[b] .. first[b] + count - 1 of each sequence in fp16, [B, count, Hkv, 128]; total[b]: rows that it has.  Rows past them are 0. */
+int smh_kv8_append(const void *q, const void *k, const void *v, void *q_out, int T, int B, int H, int Hkv, int D, long q_stride, long k_stride, long v_stride,
+                   const void *cos_tab, const void *sin_tab, int table_rows, const int32_t *lens, const int32_t *cu, int max_new, void *codes_k, void *codes_v, void *scales,
+                   void *open_k, void *open_v, const int32_t *pages, long n_pages, long pages_stride, int pages_cols, smh_stream_t stream);
+size_t smh_kv8_attn_workspace_bytes(int T, int B, int H, int Hkv, int max_new, long max_len, int window, int sinks);
+int smh_kv8_attn(const void *q, void *out, int T, int B, int H, int Hkv, int D, long q_stride, const int32_t *lens, const int32_t *cu, int max_new, long max_len, int window, int sinks,
+                 const void *codes_k, const void *codes_v, const void *scales, const void *open_k, const void *open_v, const int32_t *pages, long n_pages, long pages_stride,
+                 int pages_cols, void *workspace, size_t workspace_bytes, smh_stream_t stream);
+int smh_kv8_rows(void *out_k, void *out_v, int B, int Hkv, int D, const int32_t *total, const int32_t *first, int count, const void *codes_k, const void *codes_v, const void *scales,
+                 const void *open_k, const void *open_v, const int32_t *pages, long n_pages, long pages_stride, int pages_cols, smh_stream_t stream);
+
+/* ---- beam search ---------------------------------------------------------------------------------------------------------
+ * The other search next to the tree sampler (the reference has only the latter, mcts.py:67-182).
+ * smh_beam_select    G groups of W beams, W <= 64: of all continuations (beam r, token t) of a group the n <= 128 with the largest
+ *                    scores[r] + x[r, t] - log(sum over t' of exp(x[r, t'])), in descending order, equal ones by (r, t).  logits fp16 [G * W, ld], scores fp32 [G * W], out_scores
+ *                    fp32, out_parents int32 (r within the group), out_tokens int64, out_ended uint8 [G, n].  ended uint8 [G * W] or NULL: an ended beam has one
+ *                    continuation, eos, with its score unchanged; out_ended: the beam had ended or the token is eos.  A logit of -infinity forbids a token (one of +infinity counts as 65536), a score of
+ *                    -infinity a beam (NaN counts as that): their continuations come last, by (r, t).  Compared in 64 bits on sums of fp32 terms.
+ *                    workspace: smh_beam_select_workspace_bytes(...) bytes, any contents, 8-byte aligned; calls that overlap need one each.
+ * smh_beam_reorder   row g * W + i of each of up to 16 tensors takes the contents of row g * W + parents[g, i] (int32, cut to 0 .. W - 1), in place.  tensors, strides
+ *                    (bytes between rows), bytes (of a row that move) and units are host arrays; units[k] > 0: only the first *upto (int32 on the device) entries of
+ *                    units[k] bytes move, e.g. the page ids of rows written so far.  Multiples of 4 bytes. */
+size_t smh_beam_select_workspace_bytes(int G, int W, int vocab, int n);
+int smh_beam_select(const void *logits, long ld, const float *scores, const uint8_t *ended, int G, int W, int vocab, int n, int64_t eos, float *out_scores, int32_t *out_parents,
+                    int64_t *out_tokens, uint8_t *out_ended, void *workspace, size_t workspace_bytes, smh_stream_t stream);
+int smh_beam_reorder(const int32_t *parents, int G, int W, int n, void *const *tensors, const long *strides, const long *bytes, const int *units, const int32_t *upto,
+                     smh_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -119,6 +119,15 @@ SIGNATURES = {
     "smh_decode_stack": (c_int, [_P, c_int, _PASS, _P, c_size_t, _P]),
     "smh_decode_stack_of": (c_int, [_P, c_int, _PASS, _P, c_size_t, c_int, c_int, _P]),
     "smh_decode_finish": (c_int, [_LAYER, _PASS, _P, c_float, _P, _P]),
+    "smh_kv8_append": (c_int, [_P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_long, c_long, c_long, _P, _P, c_int, _P, _P, c_int,
+                               _P, _P, _P, _P, _P, _P, c_long, c_long, c_int, _P]),
+    "smh_kv8_attn_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_long, c_int, c_int]),
+    "smh_kv8_attn": (c_int, [_P, _P, c_int, c_int, c_int, c_int, c_int, c_long, _P, _P, c_int, c_long, c_int, c_int, _P, _P, _P, _P, _P, _P, c_long, c_long, c_int,
+                             _P, c_size_t, _P]),
+    "smh_kv8_rows": (c_int, [_P, _P, c_int, c_int, c_int, _P, _P, c_int, _P, _P, _P, _P, _P, _P, c_long, c_long, c_int, _P]),
+    "smh_beam_select_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "smh_beam_select": (c_int, [_P, c_long, _P, _P, c_int, c_int, c_int, c_int, ctypes.c_int64, _P, _P, _P, _P, _P, c_size_t, _P]),
+    "smh_beam_reorder": (c_int, [_P, c_int, c_int, c_int, _P, _P, _P, _P, _P, _P]),
     "smh_page_fork": (c_int, [_P, c_int, c_long, c_int, c_int, c_int, c_int, _P]),
 }
 

@@ -1,0 +1,545 @@
+// Attention of new rows over the paged 8-bit cache (kv8.hpp has its format).
+//
+//   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(s_j - m),  s_j = log2(e) / sqrt(128) * scale_k * (q . u_j)
+//
+// over the rows j <= place of the query and, with a window, j > place - window or j < sinks.  The queries that share a kv head (n_rep of each new row) are
+// the columns of both products, S^T = U_k Q^T and O^T = U_v^T P^T (v_mfma_f32_16x16x32_f16): codes are exact in fp16, a block's scale multiplies the fp32
+// scores, and for V the fp32 sums of the block, so that the one thing rounded below 32 bits is p, to fp16 (half a step: 2^-11 of each weight).
+// Softmax state (m, l) and sums are fp32; the running form lets a block be read once.
+//
+// Bound: HBM for a few queries a head (256 bytes a row and kv head), the matrix cores for many.
+#include "kv8.hpp"
+
+namespace smh {
+
+struct Kv8AttnParams {
+    const half_t *q;
+    half_t *out;
+    long q_stride;
+    const int32_t *lens, *cu;
+    Kv8Cache c;
+    int T, B, H, Hkv, max_new, window, sinks, splits;
+    float *part_o;                                 // [splits][T * H][128], not normalised
+    float2 *part_ml;                               // [splits][T * H]
+};
+
+// What a run of rows sees of its sequence: blocks 0 .. sink_blocks - 1 and first .. last, `count` in all, of which the last may be the open one.
+struct Kv8Span {
+    int whole, open_rows;                          // whole blocks, rows of the open one
+    int sink_blocks, first, count;
+    __device__ __forceinline__ int block(int i) const { return i < sink_blocks ? i : first + i - sink_blocks; }
+};
+__device__ __forceinline__ Kv8Span kv8_span(const Kv8AttnParams &p, const Kv8Seq &s, int lo, int hi) {      // lo, hi: places of the first and last query
+    Kv8Span v;
+    const int total = min(s.old + s.n, p.c.cols * KV8_ROWS + 63);
+    v.whole = total >> 6;
+    v.open_rows = total & 63;
+    const int last = min(hi, total - 1) >> 6;
+    v.first = 0;
+    v.sink_blocks = 0;
+    if (p.window > 0) {
+        v.first = min(max(lo - p.window + 1, 0) >> 6, last + 1);
+        v.sink_blocks = min(min((p.sinks + 63) >> 6, v.first), last + 1);
+    }
+    v.count = v.sink_blocks + last - v.first + 1;
+    return v;
+}
+
+// A wave's queries: QT tiles of 16 columns, lane l has column l % 16.
+template <int QT>
+struct Kv8Wave {
+    h8 q[QT][4];
+    f4 o[QT][8];
+    float m[QT], l[QT];                            // l: of the lane's own rows
+    int at[QT];                                    // place of the query, -1: none
+    int lo, hi;                                    // least and largest place of the wave's queries
+
+    __device__ __forceinline__ void init(const Kv8AttnParams &p, const Kv8Seq &s, int kvh, int row0, int n_rep) {
+        const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, rows = s.n * n_rep;
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            const int r = row0 + t * 16 + col;
+            const int i = r / n_rep;
+            at[t] = r < rows ? s.old + i : -1;
+            const half_t *src = p.q + (long)(s.t0 + i) * p.q_stride + (long)(kvh * n_rep + r - i * n_rep) * KV8_DIM;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) q[t][k] = r < rows ? *reinterpret_cast<const h8 *>(src + (k >> 1) * 64 + g * 16 + (k & 1) * 8) : h8{0, 0, 0, 0, 0, 0, 0, 0};
+            m[t] = -INFINITY;
+            l[t] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < 8; ++d) o[t][d] = f4{0, 0, 0, 0};
+        }
+        lo = s.old + row0 / n_rep;
+        hi = s.old + min(row0 + QT * 16 - 1, rows - 1) / n_rep;
+    }
+
+    // Scores of 64 rows -> weights, as the second product takes them.  masked: some row of the block may be out of some query's sight.  seen[t]: the lane's
+    // query sees a row of the block.
+    __device__ __forceinline__ void softmax(f4 (&x)[QT][4], float scale, int block, bool masked, int limit, int window, int sinks, h8 (&w)[QT][2], bool (&seen)[QT]) {
+        const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            seen[t] = true;
+            if (masked) {
+                const int top = min(at[t], limit - 1) - block * KV8_ROWS, low = window > 0 ? at[t] - window - block * KV8_ROWS : -1, first = sinks - block * KV8_ROWS;
+                seen[t] = top >= 0 && (low < 63 || first > 0);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = k * 16 + g * 4 + i;
+                        x[t][k][i] = r <= top && (r > low || r < first) ? x[t][k][i] * scale : -INFINITY;
+                    }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[t][k] *= scale;
+            }
+            float top = x[t][0][0];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top = fmaxf(top, x[t][k][i]);
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float now = fmaxf(m[t], top), zero = now == -INFINITY ? 0.0f : now;      // (nothing seen yet: weights of 0, not of -inf + inf)
+            if (__any(now > m[t])) {
+                const float by = __builtin_amdgcn_exp2f(m[t] - zero);
+                l[t] *= by;
+#pragma unroll
+                for (int d = 0; d < 8; ++d) o[t][d] *= by;
+                m[t] = now;
+            }
+            float sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float e = __builtin_amdgcn_exp2f(x[t][k][i] - zero);
+                    sum += e;
+                    w[t][k >> 1][(k & 1) * 4 + i] = (half_t)e;
+                }
+            l[t] += sum;
+        }
+    }
+
+    // l over the lane groups that share a query.  Scores that are all NaN leave no maximum: the lowest number stands in, so that the NaN in l is not passed over.
+    __device__ __forceinline__ void finish() {
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            l[t] += __shfl_xor(l[t], 16, 64);
+            l[t] += __shfl_xor(l[t], 32, 64);
+            if (l[t] != l[t] && m[t] == -INFINITY) m[t] = -3.0e38f;
+        }
+    }
+};
+
+__device__ __forceinline__ bool kv8_masked(const Kv8AttnParams &p, int block, int lo, int hi, int rows) {
+    if (block * KV8_ROWS + 63 > lo || rows < KV8_ROWS) return true;
+    return p.window > 0 && block * KV8_ROWS <= hi - p.window && (block + 1) * KV8_ROWS > p.sinks;
+}
+
+constexpr float KV8_SCORE_SCALE = 0.08838834764831845f * 1.4426950408889634f;       // log2(e) / sqrt(128)
+
+// The open block from memory: fp16 values, rows past its end absent.
+template <int QT>
+__device__ __forceinline__ void kv8_open_block(Kv8Wave<QT> &w, const Kv8AttnParams &p, const half_t *k, const half_t *v, int block, int rows) {
+    const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+    f4 x[QT][4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        h8 a[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) a[s] = *reinterpret_cast<const h8 *>(k + (t * 16 + col) * KV8_DIM + (s >> 1) * 64 + g * 16 + (s & 1) * 8);
+#pragma unroll
+        for (int u = 0; u < QT; ++u) {
+            x[u][t] = f4{0, 0, 0, 0};
+#pragma unroll
+            for (int s = 0; s < 4; ++s) x[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[s], w.q[u][s], x[u][t], 0, 0, 0);
+        }
+    }
+    h8 pr[QT][2];
+    bool seen[QT];
+    w.softmax(x, KV8_SCORE_SCALE, block, true, block * KV8_ROWS + rows, p.window, p.sinks, pr, seen);
+#pragma unroll
+    for (int d = 0; d < 8; ++d) {
+        h8 a[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            a[u] = *reinterpret_cast<const h8 *>(v + (d * 16 + col) * KV8_ROWS + g * 16 + u * 8);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (u * 32 + (i >> 2) * 16 + g * 4 + (i & 3) >= rows) a[u][i] = (half_t)0.0f;      // (what is there may be anything)
+        }
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            f4 s = {0, 0, 0, 0};
+#pragma unroll
+            for (int u = 0; u < 2; ++u) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[u], pr[t][u], s, 0, 0, 0);
+            if (seen[t]) w.o[t][d] += s;
+        }
+    }
+}
+
+// ---- up to 64 queries a sequence and kv head ------------------------------------------------------------------------------------
+// The four waves of a workgroup take alternate blocks of their part of the sequence, each for all queries, straight from memory into the operands; their states
+// meet in LDS.
+template <int QT>
+__global__ __launch_bounds__(256) void kv8_attn_few_kernel(Kv8AttnParams p) {
+    extern __shared__ float lds[];
+    const int kvh = blockIdx.x, split = blockIdx.y, b = blockIdx.z;
+    const Kv8Seq s = kv8_seq(p.lens, p.cu, b, p.T, p.max_new);
+    if (s.n == 0) return;
+    const int n_rep = p.H / p.Hkv, lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Kv8Wave<QT> w;
+    w.init(p, s, kvh, 0, n_rep);
+    const Kv8Span v = kv8_span(p, s, w.lo, w.hi);
+    const int per = (v.count + p.splits - 1) / p.splits, begin = split * per, end = min(begin + per, v.count);
+    const bool has_open = v.count > 0 && v.open_rows > 0 && v.block(v.count - 1) == v.whole;
+    const int end8 = min(end, v.count - (has_open ? 1 : 0));
+    const int32_t *pages = p.c.pages + (long)b * p.c.pages_stride;
+    auto tile_of = [&](int i) { return min(max((long)pages[v.block(i)], 0L), p.c.n_pages - 1) * p.Hkv + kvh; };
+
+    u32x4 kw[4][2], vw[8];
+    auto ask_k = [&](long tile) {
+        const uint8_t *k = p.c.k + tile * KV8_TILE + col * KV8_DIM + g * 16;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) kw[t][h] = *reinterpret_cast<const u32x4 *>(k + t * 16 * KV8_DIM + h * 64);
+    };
+    int i = begin + wave;
+    long tile = 0;
+    float2 sc = make_float2(0, 0);
+    if (i < end8) {
+        tile = tile_of(i);
+        ask_k(tile);
+        sc = *reinterpret_cast<const float2 *>(p.c.scales + tile * 2);
+    }
+    for (; i < end8; i += 4) {
+        const uint8_t *vp = p.c.v + tile * KV8_TILE + col * KV8_ROWS + g * 16;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) vw[d] = *reinterpret_cast<const u32x4 *>(vp + d * 16 * KV8_ROWS);
+        f4 x[QT][4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int u = 0; u < QT; ++u) x[u][t] = f4{0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const h8 a = kv8_codes8(kw[t][k >> 1][(k & 1) * 2], kw[t][k >> 1][(k & 1) * 2 + 1]);
+#pragma unroll
+                for (int u = 0; u < QT; ++u) x[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, w.q[u][k], x[u][t], 0, 0, 0);
+            }
+        }
+        const float2 sc_now = sc;
+        const int block = v.block(i);
+        if (i + 4 < end8) {
+            tile = tile_of(i + 4);
+            ask_k(tile);
+            sc = *reinterpret_cast<const float2 *>(p.c.scales + tile * 2);
+        }
+        h8 pr[QT][2];
+        bool seen[QT];
+        w.softmax(x, sc_now.x * KV8_SCORE_SCALE, block, kv8_masked(p, block, w.lo, w.hi, KV8_ROWS), (block + 1) * KV8_ROWS, p.window, p.sinks, pr, seen);
+        float by[QT];
+#pragma unroll
+        for (int t = 0; t < QT; ++t) by[t] = seen[t] ? sc_now.y : 0.0f;      // (a scale that is not finite reaches those who see the block)
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+            const h8 a0 = kv8_codes8(vw[d][0], vw[d][1]), a1 = kv8_codes8(vw[d][2], vw[d][3]);
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+                f4 sum = {0, 0, 0, 0};
+                sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, pr[t][0], sum, 0, 0, 0);
+                sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, pr[t][1], sum, 0, 0, 0);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w.o[t][d][e] = __builtin_fmaf(sum[e], by[t], w.o[t][d][e]);
+            }
+        }
+    }
+    if (has_open && v.count - 1 >= begin && v.count - 1 < end && ((v.count - 1 - begin) & 3) == wave) {
+        const long head = (long)b * p.Hkv + kvh;
+        kv8_open_block<QT>(w, p, p.c.open_k + head * KV8_TILE, p.c.open_v + head * KV8_TILE, v.whole, v.open_rows);
+    }
+    w.finish();
+    // the waves' states: [wave][16 queries][128 + 4] and (m, l)
+    constexpr int PITCH = KV8_DIM + 4;
+    float *lo = lds;
+    float2 *ml = reinterpret_cast<float2 *>(lds + 4 * 16 * PITCH);
+    const int row = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * 8;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        if (t > 0) __syncthreads();
+#pragma unroll
+        for (int d = 0; d < 8; ++d) *reinterpret_cast<f4 *>(lo + (wave * 16 + col) * PITCH + d * 16 + g * 4) = w.o[t][d];
+        if (g == 0) ml[wave * 16 + col] = make_float2(w.m[t], w.l[t]);
+        __syncthreads();
+        const int r = t * 16 + row;
+        if (r >= s.n * n_rep) continue;
+        float top = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) top = fmaxf(top, ml[k * 16 + row].x);
+        const float zero = top == -INFINITY ? 0.0f : top;
+        f4 a = {0, 0, 0, 0}, c = {0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float by = __builtin_amdgcn_exp2f(ml[k * 16 + row].x - zero);
+            l += ml[k * 16 + row].y * by;
+            a += *reinterpret_cast<const f4 *>(lo + (k * 16 + row) * PITCH + d0) * by;
+            c += *reinterpret_cast<const f4 *>(lo + (k * 16 + row) * PITCH + d0 + 4) * by;
+        }
+        const int tok = r / n_rep;
+        const long out = (long)(s.t0 + tok) * p.H + kvh * n_rep + r - tok * n_rep;
+        if (p.splits == 1) {
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            h8 y;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { y[e] = (half_t)(a[e] * inv); y[4 + e] = (half_t)(c[e] * inv); }
+            *reinterpret_cast<h8 *>(p.out + out * KV8_DIM + d0) = y;
+        } else {
+            const long at = (long)split * p.T * p.H + out;
+            if ((threadIdx.x & 15) == 0) p.part_ml[at] = make_float2(top, l);
+            if (top != -INFINITY) {
+                *reinterpret_cast<f4 *>(p.part_o + at * KV8_DIM + d0) = a;
+                *reinterpret_cast<f4 *>(p.part_o + at * KV8_DIM + d0 + 4) = c;
+            }
+        }
+    }
+}
+
+// ---- many queries -------------------------------------------------------------------------------------------------------------
+// Four waves have QT * 16 queries each and go through the same blocks; a block's codes become fp16 once for all of them, in LDS, in the order in which the lanes
+// read their operands (1 KB a read, no bank twice).
+template <int QT>
+__global__ __launch_bounds__(256) void kv8_attn_many_kernel(Kv8AttnParams p) {
+    extern __shared__ float lds[];
+    h8 *kl = reinterpret_cast<h8 *>(lds), *vl = kl + 1024;             // [tile][k step][lane], [dims of 16][half][lane]
+    const int kvh = blockIdx.x % p.Hkv, b = blockIdx.x / p.Hkv, split = blockIdx.z;
+    const Kv8Seq s = kv8_seq(p.lens, p.cu, b, p.T, p.max_new);
+    const int n_rep = p.H / p.Hkv, rows = s.n * n_rep;
+    const int row0 = (gridDim.y - 1 - blockIdx.y) * (QT * 64);         // (the last queries have the most to see: they begin first)
+    if (row0 >= rows) return;
+    const int t = threadIdx.x, lane = t & 63, col = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    Kv8Wave<QT> w;
+    w.init(p, s, kvh, row0 + wave * QT * 16, n_rep);
+    const bool idle = row0 + wave * QT * 16 >= rows;
+    const Kv8Span v = kv8_span(p, s, s.old + row0 / n_rep, s.old + min(row0 + QT * 64 - 1, rows - 1) / n_rep);
+    const int per = (v.count + p.splits - 1) / p.splits, begin = split * per, end = min(begin + per, v.count);
+    const bool has_open = v.count > 0 && v.open_rows > 0 && v.block(v.count - 1) == v.whole;
+    const int end8 = min(end, v.count - (has_open ? 1 : 0));
+    const int32_t *pages = p.c.pages + (long)b * p.c.pages_stride;
+    auto tile_of = [&](int i) { return min(max((long)pages[v.block(i)], 0L), p.c.n_pages - 1) * p.Hkv + kvh; };
+    u32x4 kw[2], vw[2];
+    auto ask = [&](long tile) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {                                  // wave: tile of 16 rows; two halves of their dims
+            kw[h] = *reinterpret_cast<const u32x4 *>(p.c.k + tile * KV8_TILE + (wave * 16 + col) * KV8_DIM + h * 64 + g * 16);
+            vw[h] = *reinterpret_cast<const u32x4 *>(p.c.v + tile * KV8_TILE + ((wave * 2 + h) * 16 + col) * KV8_ROWS + g * 16);
+        }
+    };
+    float2 sc = make_float2(0, 0);
+    if (begin < end8) {
+        const long tile = tile_of(begin);
+        ask(tile);
+        sc = *reinterpret_cast<const float2 *>(p.c.scales + tile * 2);
+    }
+    for (int i = begin; i < end8; ++i) {
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                kl[(wave * 4 + h * 2 + e) * 64 + lane] = kv8_codes8(kw[h][e * 2], kw[h][e * 2 + 1]);
+                vl[((wave * 2 + h) * 2 + e) * 64 + lane] = kv8_codes8(vw[h][e * 2], vw[h][e * 2 + 1]);
+            }
+        const float2 sc_now = sc;
+        const int block = v.block(i);
+        if (i + 1 < end8) {
+            const long tile = tile_of(i + 1);
+            ask(tile);
+            sc = *reinterpret_cast<const float2 *>(p.c.scales + tile * 2);
+        }
+        __syncthreads();
+        if (idle || block * KV8_ROWS > w.hi) continue;                 // (nothing there for this wave)
+        f4 x[QT][4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+#pragma unroll
+            for (int u = 0; u < QT; ++u) x[u][k] = f4{0, 0, 0, 0};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const h8 a = kl[(k * 4 + e) * 64 + lane];
+#pragma unroll
+                for (int u = 0; u < QT; ++u) x[u][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, w.q[u][e], x[u][k], 0, 0, 0);
+            }
+        }
+        h8 pr[QT][2];
+        bool seen[QT];
+        w.softmax(x, sc_now.x * KV8_SCORE_SCALE, block, kv8_masked(p, block, w.lo, w.hi, KV8_ROWS), (block + 1) * KV8_ROWS, p.window, p.sinks, pr, seen);
+        float by[QT];
+#pragma unroll
+        for (int u = 0; u < QT; ++u) by[u] = seen[u] ? sc_now.y : 0.0f;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+            const h8 a0 = vl[(d * 2) * 64 + lane], a1 = vl[(d * 2 + 1) * 64 + lane];
+#pragma unroll
+            for (int u = 0; u < QT; ++u) {
+                f4 sum = {0, 0, 0, 0};
+                sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, pr[u][0], sum, 0, 0, 0);
+                sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, pr[u][1], sum, 0, 0, 0);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w.o[u][d][e] = __builtin_fmaf(sum[e], by[u], w.o[u][d][e]);
+            }
+        }
+    }
+    if (idle) return;
+    if (has_open && v.count - 1 >= begin && v.count - 1 < end && v.whole * KV8_ROWS <= w.hi) {
+        const long head = (long)b * p.Hkv + kvh;
+        kv8_open_block<QT>(w, p, p.c.open_k + head * KV8_TILE, p.c.open_v + head * KV8_TILE, v.whole, v.open_rows);
+    }
+    w.finish();
+#pragma unroll
+    for (int u = 0; u < QT; ++u) {
+        const int r = row0 + (wave * QT + u) * 16 + col;
+        if (r >= rows) continue;
+        const int tok = r / n_rep;
+        const long out = (long)(s.t0 + tok) * p.H + kvh * n_rep + r - tok * n_rep;
+        if (p.splits == 1) {
+            const float inv = w.l[u] == 0.0f ? 0.0f : 1.0f / w.l[u];
+#pragma unroll
+            for (int d = 0; d < 8; ++d) {
+                h4 y;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = (half_t)(w.o[u][d][e] * inv);
+                *reinterpret_cast<h4 *>(p.out + out * KV8_DIM + d * 16 + g * 4) = y;
+            }
+        } else {
+            const long at = (long)split * p.T * p.H + out;
+            if (g == 0) p.part_ml[at] = make_float2(w.m[u], w.l[u]);
+            if (w.m[u] != -INFINITY) {
+#pragma unroll
+                for (int d = 0; d < 8; ++d) *reinterpret_cast<f4 *>(p.part_o + at * KV8_DIM + d * 16 + g * 4) = w.o[u][d];
+            }
+        }
+    }
+}
+
+// The parts of each query: half a wave a query, four dims a lane.
+__global__ __launch_bounds__(256) void kv8_attn_merge_kernel(Kv8AttnParams p) {
+    const long rows = (long)p.T * p.H, r = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (r >= rows) return;
+    if (p.cu != nullptr) {                         // rows of no sequence (behind the last one, past max_new) have no parts
+        const int tok = (int)(r / p.H);
+        int lo = 0, hi = p.B;                      // the last sequence that begins at or before the row
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (p.cu[mid] <= tok) lo = mid;
+            else hi = mid;
+        }
+        const Kv8Seq s = kv8_seq(p.lens, p.cu, lo, p.T, p.max_new);
+        if (tok < s.t0 || tok >= s.t0 + s.n) return;
+    }
+    const int d = (threadIdx.x & 31) * 4;
+    float top = -INFINITY, l = 0.0f;
+    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, p.part_ml[s * rows + r].x);
+    const float zero = top == -INFINITY ? 0.0f : top;
+    f4 a = {0, 0, 0, 0};
+    for (int s = 0; s < p.splits; ++s) {
+        const float2 ml = p.part_ml[s * rows + r];
+        if (ml.x == -INFINITY) continue;           // (no sums were left)
+        const float by = __builtin_amdgcn_exp2f(ml.x - zero);
+        l += ml.y * by;
+        a += *reinterpret_cast<const f4 *>(p.part_o + (s * rows + r) * KV8_DIM + d) * by;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    h4 y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = (half_t)(a[e] * inv);
+    *reinterpret_cast<h4 *>(p.out + r * KV8_DIM + d) = y;
+}
+
+}  // namespace smh
+
+using namespace smh;
+
+namespace {
+struct Kv8Plan { int tiles, splits; long groups; };        // tiles of 16 queries a workgroup (0: many), parts of a sequence
+// Blocks that a sequence of up to max_len rows shows its queries, from above
+long kv8_blocks(int max_new, long max_len, int window, int sinks) {
+    long n = (max_len + 63) / 64;
+    if (window > 0) {
+        const long w = ((long)window + max_new + 62) / 64 + 1 + (sinks + 63) / 64;
+        n = n < w ? n : w;
+    }
+    return n < 1 ? 1 : n;
+}
+Kv8Plan kv8_plan(int B, int H, int Hkv, int max_new, long max_len, int window, int sinks) {
+    const long rows = (long)max_new * (H / Hkv), blocks = kv8_blocks(max_new, max_len, window, sinks);
+    Kv8Plan p;
+    p.tiles = rows <= 64 ? (int)((rows + 15) / 16) : 0;
+    p.groups = p.tiles ? 1 : (rows + 127) / 128;
+    const long base = (long)B * Hkv * p.groups, want = p.tiles ? 1024 : 512, least = p.tiles ? 4 : 8;
+    long s = (want + base - 1) / base;
+    const long most = (blocks + least - 1) / least;
+    s = s < most ? s : most;
+    p.splits = (int)(s < 1 ? 1 : s > 256 ? 256 : s);
+    return p;
+}
+bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+}  // namespace
+
+extern "C" size_t smh_kv8_attn_workspace_bytes(int T, int B, int H, int Hkv, int max_new, long max_len, int window, int sinks) {
+    if (T < 1 || B < 1 || Hkv < 1 || H < Hkv || H % Hkv != 0 || max_new < 1 || max_len < 1 || window < 0 || sinks < 0) return 0;
+    const Kv8Plan p = kv8_plan(B, H, Hkv, max_new < T ? max_new : T, max_len, window, sinks);
+    return p.splits == 1 ? 0 : (size_t)p.splits * T * H * (KV8_DIM + 2) * sizeof(float);
+}
+
+extern "C" int smh_kv8_attn(const void *q, void *out, int T, int B, int H, int Hkv, int D, long q_stride, const int32_t *lens, const int32_t *cu, int max_new, long max_len, int window,
+                            int sinks, const void *codes_k, const void *codes_v, const void *scales, const void *open_k, const void *open_v, const int32_t *pages, long n_pages,
+                            long pages_stride, int pages_cols, void *workspace, size_t workspace_bytes, smh_stream_t stream) {
+    SMH_REQUIRE(D == KV8_DIM, "smh_kv8_attn: head dim %d (only 128)", D);
+    SMH_REQUIRE(B >= 1 && B <= 65535 && Hkv >= 1 && Hkv <= 4096 && H >= Hkv && H % Hkv == 0 && H <= 65535, "smh_kv8_attn: B=%d (1 .. 65535) H=%d Hkv=%d (1 .. 4096)", B, H, Hkv);
+    SMH_REQUIRE(T >= 0 && max_new >= 0 && max_new <= KV8_MAX_LEN && max_len >= 1 && window >= 0 && window <= KV8_MAX_LEN && sinks >= 0 && sinks <= KV8_MAX_LEN,
+                "smh_kv8_attn: T=%d max_new=%d max_len=%ld window=%d sinks=%d", T, max_new, max_len, window, sinks);
+    SMH_REQUIRE(cu || T == B, "smh_kv8_attn: without cu every sequence has one row: T=%d B=%d", T, B);
+    SMH_REQUIRE(q_stride >= (long)H * D && q_stride % 8 == 0, "smh_kv8_attn: token stride %ld", q_stride);
+    SMH_REQUIRE(codes_k && codes_v && scales && open_k && open_v && pages, "smh_kv8_attn: null pointer in the cache");
+    SMH_REQUIRE(aligned16(codes_k) && aligned16(codes_v) && aligned16(open_k) && aligned16(open_v) && ((uintptr_t)scales & 7) == 0,
+                "smh_kv8_attn: the cache's tensors are 16-byte aligned, its scales 8");
+    SMH_REQUIRE(n_pages >= 1 && pages_cols >= 0 && pages_cols <= KV8_MAX_LEN / KV8_ROWS - 1 && pages_stride >= pages_cols, "smh_kv8_attn: n_pages=%ld pages_cols=%d (at most %d) pages_stride=%ld",
+                n_pages, pages_cols, KV8_MAX_LEN / KV8_ROWS - 1, pages_stride);
+    if (T == 0 || max_new == 0) return 0;
+    SMH_REQUIRE(q && out && lens, "smh_kv8_attn: null pointer");
+    SMH_REQUIRE(aligned16(q) && aligned16(out), "smh_kv8_attn: tensors are 16-byte aligned");
+    const int most = cu ? (max_new < T ? max_new : T) : 1;
+    const Kv8Plan plan = kv8_plan(B, H, Hkv, most, max_len, window, sinks);
+    Kv8AttnParams p{(const half_t *)q, (half_t *)out, q_stride, lens, cu,
+                    {(uint8_t *)codes_k, (uint8_t *)codes_v, (float *)scales, (half_t *)open_k, (half_t *)open_v, pages, pages_stride, n_pages, pages_cols},
+                    T, B, H, Hkv, most, window, sinks, plan.splits, nullptr, nullptr};
+    if (plan.splits > 1) {
+        const size_t need = (size_t)plan.splits * T * H * (KV8_DIM + 2) * sizeof(float);
+        SMH_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need, "smh_kv8_attn: workspace of %zu bytes, %zu needed (16-byte aligned)", workspace_bytes, need);
+        p.part_o = (float *)workspace;
+        p.part_ml = (float2 *)(p.part_o + (size_t)plan.splits * T * H * KV8_DIM);
+    }
+    const hipStream_t st = (hipStream_t)stream;
+    if (plan.tiles) {
+        const dim3 grid(Hkv, plan.splits, B);
+        const size_t bytes = 4 * 16 * (KV8_DIM + 4) * 4 + 64 * 8;
+        if (plan.tiles == 1) hipLaunchKernelGGL(kv8_attn_few_kernel<1>, grid, dim3(256), bytes, st, p);
+        else if (plan.tiles == 2) hipLaunchKernelGGL(kv8_attn_few_kernel<2>, grid, dim3(256), bytes, st, p);
+        else if (plan.tiles == 3) hipLaunchKernelGGL(kv8_attn_few_kernel<3>, grid, dim3(256), bytes, st, p);
+        else hipLaunchKernelGGL(kv8_attn_few_kernel<4>, grid, dim3(256), bytes, st, p);
+    } else {
+        SMH_REQUIRE((long)B * Hkv < (1L << 31) && plan.groups <= 65535, "smh_kv8_attn: max_new=%d with %d queries a kv head (at most 65535 groups of 128)", max_new, H / Hkv);
+        hipLaunchKernelGGL(kv8_attn_many_kernel<2>, dim3(B * Hkv, (unsigned)plan.groups, plan.splits), dim3(256), 32768, st, p);
+    }
+    if (int rc = launch_status()) return rc;
+    if (plan.splits == 1) return 0;
+    const long rows = (long)T * H;
+    SMH_REQUIRE((rows + 7) / 8 < (1L << 31), "smh_kv8_attn: T=%d", T);
+    hipLaunchKernelGGL(kv8_attn_merge_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, p);
+    return launch_status();
+}

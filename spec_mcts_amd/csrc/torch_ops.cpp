@@ -33,6 +33,13 @@ struct Api {
     decltype(&smh_paged_attn_workspace_bytes) paged_bytes;
     decltype(&smh_shared_prefix_attn) shared_attn;
     decltype(&smh_paged_prefix_attn) paged_attn;
+    decltype(&smh_kv8_append) kv8_append;
+    decltype(&smh_kv8_attn_workspace_bytes) kv8_attn_bytes;
+    decltype(&smh_kv8_attn) kv8_attn;
+    decltype(&smh_kv8_rows) kv8_rows;
+    decltype(&smh_beam_select_workspace_bytes) beam_select_bytes;
+    decltype(&smh_beam_select) beam_select;
+    decltype(&smh_beam_reorder) beam_reorder;
 } api;
 PyObject *smh_error = nullptr;
 
@@ -452,6 +459,241 @@ PyObject *layer_state(Args x) {
     return PyLong_FromLong(same ? rows : -1 - rows);
 }
 
+// ---- the paged 8-bit cache and beam search (kernels.py: kv8_append, kv8_attn, kv8_rows, beam_select, beam_reorder) ----
+// Types and sizes are looked at first, so that what a call refuses it refuses for tensors anywhere; then that all of them are on the current GPU.
+struct Here {
+    const at::Tensor *first = nullptr;
+    void add(const at::Tensor &t) {
+        if (first == nullptr) first = &t;
+        need(t.device() == first->device(), "all tensors must be on one device");
+    }
+    void check() const {
+        need(first->is_cuda(), "spec_mcts_amd kernels need GPU tensors (there is no CPU fallback)");
+        need(first->device().index() == c10::hip::current_device(), "the tensors' GPU must be the current device");
+    }
+};
+constexpr int64_t KV8_BLOCK = 64, KV8_D = 128;
+int small(int64_t v, const char *why) {
+    need(v >= 0 && v <= INT32_MAX, why);
+    return (int)v;
+}
+struct Cache {
+    at::Tensor codes_k, codes_v, scales, open_k, open_v, pages;
+    int64_t n_pages, Hkv, cols;
+};
+const at::Tensor &ids(PyObject *o, const char *what, int64_t n, Here &here) {
+    const at::Tensor &t = tensor(o, what);
+    if (!(is(t, at::kInt) && t.dim() == 1 && t.is_contiguous() && (n < 0 || t.size(0) == n))) refuse(std::string(what) + " must be a contiguous int32 vector of one entry a sequence (cu: one more)");
+    here.add(t);
+    return t;
+}
+Cache kv8_cache(PyObject *o, int64_t B, Here &here) {
+    PyObject *seq = made(PySequence_Fast(o, "cache is (codes_k, codes_v, scales, open_k, open_v, pages)"));
+    Cache c;
+    try {
+        need(PySequence_Fast_GET_SIZE(seq) == 6, "cache is (codes_k, codes_v, scales, open_k, open_v, pages)");
+        at::Tensor *to[6] = {&c.codes_k, &c.codes_v, &c.scales, &c.open_k, &c.open_v, &c.pages};
+        for (int i = 0; i < 6; ++i) *to[i] = tensor(PySequence_Fast_GET_ITEM(seq, i), "a member of the cache");
+    } catch (Refused &) {
+        Py_DECREF(seq);
+        throw;
+    }
+    Py_DECREF(seq);
+    need(is(c.codes_k, at::kByte) && c.codes_k.dim() == 4 && c.codes_k.size(2) == KV8_BLOCK && c.codes_k.size(3) == KV8_D, "codes_k must be uint8 [pages, kv heads, 64, 128]");
+    c.n_pages = c.codes_k.size(0);
+    c.Hkv = c.codes_k.size(1);
+    need(c.n_pages >= 1 && c.Hkv >= 1, "the cache has no pages or heads");
+    need(is(c.codes_v, at::kByte) && c.codes_v.sizes() == at::IntArrayRef({c.n_pages, c.Hkv, KV8_D, KV8_BLOCK}), "codes_v must be uint8 [pages, kv heads, 128, 64]");
+    need(is(c.scales, at::kFloat) && c.scales.sizes() == at::IntArrayRef({c.n_pages, c.Hkv, 2}), "scales must be float32 [pages, kv heads, 2]");
+    need(is(c.open_k, at::kHalf) && c.open_k.dim() == 4 && c.open_k.size(0) >= B && c.open_k.sizes().slice(1) == at::IntArrayRef({c.Hkv, KV8_BLOCK, KV8_D}),
+         "open_k must be fp16 [sequences, kv heads, 64, 128]");
+    need(is(c.open_v, at::kHalf) && c.open_v.dim() == 4 && c.open_v.size(0) >= B && c.open_v.sizes().slice(1) == at::IntArrayRef({c.Hkv, KV8_D, KV8_BLOCK}),
+         "open_v must be fp16 [sequences, kv heads, 128, 64]");
+    need(c.codes_k.is_contiguous() && c.codes_v.is_contiguous() && c.scales.is_contiguous() && c.open_k.is_contiguous() && c.open_v.is_contiguous(), "the cache's tensors must be contiguous");
+    need(is(c.pages, at::kInt) && c.pages.dim() == 2 && c.pages.size(0) >= B && (c.pages.size(1) <= 1 || c.pages.stride(1) == 1) && c.pages.stride(0) >= c.pages.size(1),
+         "pages must be int32 [sequences, blocks], blocks contiguous");
+    c.cols = c.pages.size(1);
+    for (const at::Tensor *t : {&c.codes_k, &c.codes_v, &c.scales, &c.open_k, &c.open_v, &c.pages}) here.add(*t);
+    return c;
+}
+// [T, heads, 128] fp16 with contiguous heads
+const at::Tensor &packed(PyObject *o, const char *what, Here &here) {
+    const at::Tensor &t = tensor(o, what);
+    if (!(is(t, at::kHalf) && t.dim() == 3 && t.size(2) == KV8_D && t.size(1) >= 1 && t.stride(2) == 1 && (t.size(1) == 1 || t.stride(1) == KV8_D) &&
+          (t.size(0) <= 1 || (t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1) * KV8_D))))
+        refuse(std::string(what) + " must be fp16 [rows, heads, 128] with contiguous heads and rows a multiple of 8 values apart");
+    here.add(t);
+    return t;
+}
+long row_stride(const at::Tensor &t) { return t.size(0) <= 1 ? t.size(1) * KV8_D : t.stride(0); }
+
+// (q, k, v, cos, sin, cache, lens, cu, max_new, out) -> q rotated
+PyObject *kv8_append(Args x) {
+    Here here;
+    const at::Tensor &q = packed(x[0], "q", here), &k = packed(x[1], "k", here), &v = packed(x[2], "v", here);
+    const at::Tensor &cos = tensor(x[3], "cos"), &sin = tensor(x[4], "sin");
+    need(is(cos, at::kHalf) && cos.dim() == 2 && cos.size(0) >= 1 && cos.size(1) == KV8_D / 2 && cos.is_contiguous() && is(sin, at::kHalf) && sin.sizes() == cos.sizes() && sin.is_contiguous(),
+         "cos and sin must be fp16 [places, 64]");
+    here.add(cos);
+    here.add(sin);
+    const at::Tensor &lens = ids(x[6], "lens", -1, here);
+    const int64_t B = lens.size(0), T = q.size(0), H = q.size(1);
+    const Cache c = kv8_cache(x[5], B, here);
+    need(k.size(0) == T && v.size(0) == T && k.size(1) == c.Hkv && v.size(1) == c.Hkv && H % c.Hkv == 0, "q [T, H, 128], k and v [T, kv heads, 128] of the cache's heads");
+    const int max_new = small(whole_number(x[8]), "max_new must not be negative");
+    const at::Tensor *cu = none(x[7]) ? nullptr : &ids(x[7], "cu", B + 1, here);
+    need(cu != nullptr || (T == B && max_new == 1), "without cu every sequence has one new row");
+    at::Tensor out;
+    if (none(x[9])) {
+        here.check();
+        out = empty({T, H, KV8_D}, at::kHalf, q);
+    } else {
+        out = tensor(x[9], "out");
+        need(is(out, at::kHalf) && out.sizes() == q.sizes() && out.is_contiguous(), "out must be contiguous fp16 like q");
+        here.add(out);
+        here.check();
+    }
+    if (B == 0) return give(out);
+    check(api.kv8_append(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), small(T, "T"), small(B, "B"), small(H, "H"), small(c.Hkv, "kv heads"), KV8_D, row_stride(q), row_stride(k),
+                         row_stride(v), cos.data_ptr(), sin.data_ptr(), small(cos.size(0), "the tables are too long"), lens.data_ptr<int32_t>(), cu ? cu->data_ptr<int32_t>() : nullptr, max_new,
+                         c.codes_k.data_ptr(), c.codes_v.data_ptr(), c.scales.data_ptr(), c.open_k.data_ptr(), c.open_v.data_ptr(), c.pages.data_ptr<int32_t>(), c.n_pages, c.pages.stride(0),
+                         small(c.cols, "pages has too many columns"), stream()),
+          "smh_kv8_append");
+    return give(out);
+}
+
+// (q, cache, lens, cu, max_new, max_len, window, sinks, out)
+PyObject *kv8_attn(Args x) {
+    Here here;
+    const at::Tensor &q = packed(x[0], "q", here), &lens = ids(x[2], "lens", -1, here);
+    const int64_t B = lens.size(0), T = q.size(0), H = q.size(1);
+    const Cache c = kv8_cache(x[1], B, here);
+    need(H % c.Hkv == 0, "the query heads must be a multiple of the cache's");
+    const int max_new = small(whole_number(x[4]), "max_new must not be negative");
+    const at::Tensor *cu = none(x[3]) ? nullptr : &ids(x[3], "cu", B + 1, here);
+    need(cu != nullptr || (T == B && max_new == 1), "without cu every sequence has one new row");
+    const long max_len = none(x[5]) ? c.cols * KV8_BLOCK + KV8_BLOCK - 1 : whole_number(x[5]);
+    need(max_len >= 1, "max_len must be positive");
+    const int window = small(whole_number(x[6]), "window must not be negative"), sinks = small(whole_number(x[7]), "sinks must not be negative");
+    at::Tensor out;
+    if (none(x[8])) {
+        here.check();
+        out = empty({T, H, KV8_D}, at::kHalf, q);
+    } else {
+        out = tensor(x[8], "out");
+        need(is(out, at::kHalf) && out.sizes() == q.sizes() && out.is_contiguous(), "out must be contiguous fp16 like q");
+        here.add(out);
+        here.check();
+    }
+    if (B == 0 || T == 0) return give(out);
+    const size_t bytes = api.kv8_attn_bytes(small(T, "T"), small(B, "B"), small(H, "H"), small(c.Hkv, "kv heads"), cu ? max_new : 1, max_len, window, sinks);
+    at::Tensor ws;                                 // of this call's own: a captured graph or another stream keeps its own
+    if (bytes) ws = empty({(int64_t)bytes}, at::kByte, q);
+    check(api.kv8_attn(q.data_ptr(), out.data_ptr(), (int)T, (int)B, (int)H, (int)c.Hkv, KV8_D, row_stride(q), lens.data_ptr<int32_t>(), cu ? cu->data_ptr<int32_t>() : nullptr, max_new, max_len,
+                       window, sinks, c.codes_k.data_ptr(), c.codes_v.data_ptr(), c.scales.data_ptr(), c.open_k.data_ptr(), c.open_v.data_ptr(), c.pages.data_ptr<int32_t>(), c.n_pages,
+                       c.pages.stride(0), small(c.cols, "pages has too many columns"), bytes ? ws.data_ptr() : nullptr, bytes, stream()),
+          "smh_kv8_attn");
+    return give(out);
+}
+
+// (cache, total, first, count) -> (k, v)
+PyObject *kv8_rows(Args x) {
+    Here here;
+    const at::Tensor &total = ids(x[1], "total", -1, here);
+    const int64_t B = total.size(0);
+    const at::Tensor &first = ids(x[2], "first", B, here);
+    const Cache c = kv8_cache(x[0], B, here);
+    const int count = small(whole_number(x[3]), "count must not be negative");
+    here.check();
+    at::Tensor k = empty({B, count, c.Hkv, KV8_D}, at::kHalf, total), v = at::empty_like(k);
+    if (B > 0)
+        check(api.kv8_rows(k.data_ptr(), v.data_ptr(), small(B, "B"), (int)c.Hkv, KV8_D, total.data_ptr<int32_t>(), first.data_ptr<int32_t>(), count, c.codes_k.data_ptr(), c.codes_v.data_ptr(),
+                           c.scales.data_ptr(), c.open_k.data_ptr(), c.open_v.data_ptr(), c.pages.data_ptr<int32_t>(), c.n_pages, c.pages.stride(0),
+                           small(c.cols, "pages has too many columns"), stream()),
+              "smh_kv8_rows");
+    return made(Py_BuildValue("(NN)", give(k), give(v)));
+}
+
+// (logits, scores, beams, n, ended, eos) -> (scores, parents, tokens, ended)
+PyObject *beam_select(Args x) {
+    Here here;
+    const at::Tensor &logits = tensor(x[0], "logits"), &scores = tensor(x[1], "scores");
+    need(is(logits, at::kHalf) && logits.dim() == 2 && (logits.size(1) <= 1 || logits.stride(1) == 1) && (logits.size(0) <= 1 || logits.stride(0) >= logits.size(1)),
+         "logits must be fp16 [rows, vocab], a row contiguous");
+    here.add(logits);
+    const int64_t rows = logits.size(0), vocab = logits.size(1);
+    need(is(scores, at::kFloat) && scores.dim() == 1 && scores.size(0) == rows && scores.is_contiguous(), "scores must be a contiguous float32 vector of one entry a row");
+    here.add(scores);
+    const long W = whole_number(x[2]);
+    need(W >= 1 && rows % W == 0, "the rows must be a multiple of beams");
+    const int64_t G = rows / W;
+    const long n = none(x[3]) ? W : whole_number(x[3]);
+    need(n >= 1, "n must be positive");
+    const at::Tensor *ended = nullptr;
+    if (!none(x[4])) {
+        ended = &tensor(x[4], "ended");
+        need((is(*ended, at::kByte) || is(*ended, at::kBool)) && ended->numel() == rows && ended->is_contiguous(), "ended must be uint8 or bool, one entry a row");
+        here.add(*ended);
+    }
+    const long eos = whole_number(x[5]);
+    here.check();
+    at::Tensor best = empty({G, n}, at::kFloat, logits), parents = empty({G, n}, at::kInt, logits), tokens = empty({G, n}, at::kLong, logits), done = empty({G, n}, at::kByte, logits);
+    if (G > 0) {
+        const int g = small(G, "too many groups"), w = small(W, "too many beams"), vo = small(vocab, "the vocabulary is too large"), m = small(n, "n is too large");
+        const size_t bytes = api.beam_select_bytes(g, w, vo, m);
+        at::Tensor ws = empty({(int64_t)bytes}, at::kByte, logits);
+        check(api.beam_select(logits.data_ptr(), rows <= 1 ? vocab : logits.stride(0), scores.data_ptr<float>(), ended ? (const uint8_t *)ended->data_ptr() : nullptr, g, w, vo, m, eos,
+                              best.data_ptr<float>(), parents.data_ptr<int32_t>(), tokens.data_ptr<int64_t>(), done.data_ptr<uint8_t>(), bytes ? ws.data_ptr() : nullptr, bytes, stream()),
+              "smh_beam_select");
+    }
+    return made(Py_BuildValue("(NNNN)", give(best), give(parents), give(tokens), give(done)));
+}
+
+// (parents, rows, columns, upto)
+PyObject *beam_reorder(Args x) {
+    Here here;
+    const at::Tensor &parents = tensor(x[0], "parents");
+    need(is(parents, at::kInt) && parents.dim() == 2 && parents.is_contiguous(), "parents must be contiguous int32 [groups, beams]");
+    here.add(parents);
+    const int64_t G = parents.size(0), W = parents.size(1);
+    const at::Tensor *upto = none(x[3]) ? nullptr : &ids(x[3], "upto", 1, here);
+    constexpr int MOST = 16;
+    void *at_[MOST];
+    long stride[MOST], bytes[MOST];
+    int unit[MOST], n = 0;
+    for (int part = 1; part <= 2; ++part) {
+        PyObject *seq = made(PySequence_Fast(x[part], "rows and columns are sequences of tensors"));
+        try {
+            for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(seq); ++i) {
+                const at::Tensor &t = tensor(PySequence_Fast_GET_ITEM(seq, i), "a state");
+                need(n < MOST, "at most 16 states a call");
+                const int64_t es = (int64_t)t.element_size();
+                need(t.dim() >= 1 && t.size(0) == G * W, "a state has a row for each beam");
+                need(part == 1 || (t.dim() == 2 && (es == 4 || es == 8)), "columns are 2-D tensors of 4- or 8-byte entries");
+                need(part == 1 || upto != nullptr, "columns need upto");
+                need(t.size(0) <= 1 || t.numel() == 0 || t[0].is_contiguous(), "a state's rows must be contiguous");
+                const int64_t in_row = t.size(0) ? t.numel() / t.size(0) : 0;
+                need(t.size(0) <= 1 || t.stride(0) >= in_row, "a state's rows must not overlap");
+                here.add(t);
+                at_[n] = t.data_ptr();
+                bytes[n] = in_row * es;
+                stride[n] = t.size(0) <= 1 ? bytes[n] : t.stride(0) * es;
+                unit[n] = part == 1 ? 0 : (int)es;
+                if (bytes[n] > 0) ++n;
+            }
+        } catch (...) {
+            Py_DECREF(seq);
+            throw;
+        }
+        Py_DECREF(seq);
+    }
+    here.check();
+    if (G > 0 && W > 0 && n > 0)
+        check(api.beam_reorder(parents.data_ptr<int32_t>(), small(G, "too many groups"), small(W, "too many beams"), n, at_, stride, bytes, unit, upto ? upto->data_ptr<int32_t>() : nullptr, stream()),
+              "smh_beam_reorder");
+    Py_RETURN_NONE;
+}
+
 template <PyObject *(*F)(Args), int N>
 PyObject *call(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
@@ -487,6 +729,13 @@ PyObject *connect(PyObject *, PyObject *const *args, Py_ssize_t n) {
     find(api.paged_bytes, "smh_paged_attn_workspace_bytes");
     find(api.shared_attn, "smh_shared_prefix_attn");
     find(api.paged_attn, "smh_paged_prefix_attn");
+    find(api.kv8_append, "smh_kv8_append");
+    find(api.kv8_attn_bytes, "smh_kv8_attn_workspace_bytes");
+    find(api.kv8_attn, "smh_kv8_attn");
+    find(api.kv8_rows, "smh_kv8_rows");
+    find(api.beam_select_bytes, "smh_beam_select_workspace_bytes");
+    find(api.beam_select, "smh_beam_select");
+    find(api.beam_reorder, "smh_beam_reorder");
     if (!ok) { PyErr_SetString(PyExc_RuntimeError, "the library lacks an entry point: build it again"); return nullptr; }
     Py_XDECREF(smh_error);
     smh_error = args[1];
@@ -498,7 +747,8 @@ PyObject *connect(PyObject *, PyObject *const *args, Py_ssize_t n) {
 PyMethodDef methods[] = {
     {"connect", (PyCFunction)(void (*)(void))connect, METH_FASTCALL, nullptr},
     OP(matmul_q40, 6), OP(deq_int40, 4), OP(q_int40, 1), OP(quantize_q40_t, 1), OP(sample_topk_counts, 6), OP(tree_step, 14),
-    OP(shared_prefix_attn, 15), OP(paged_prefix_attn, 15), OP(layer_state, 2), {nullptr, nullptr, 0, nullptr}};
+    OP(shared_prefix_attn, 15), OP(paged_prefix_attn, 15), OP(layer_state, 2),
+    OP(kv8_append, 10), OP(kv8_attn, 9), OP(kv8_rows, 4), OP(beam_select, 6), OP(beam_reorder, 4), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -11,7 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from typing import Dict, Optional, Sequence, Tuple
+from typing import Dict, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -1027,3 +1027,77 @@ def chunk_attn(p: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tenso
     own = p[:, offset:] if offset < L else p[:, :1]                    # a view: same table, first own page
     return paged_prefix_attn(q.contiguous(), own, lens, k, v, head_major=True, prefix_k=k, prefix_v=v, P=offset,
                              prefix_head_major=True, lens_stride=0)
+
+
+# ---------------------------------------------------------------------------------------------
+# paged 8-bit cache
+# ---------------------------------------------------------------------------------------------
+KV8_BLOCK = 64
+
+
+class KV8Cache(NamedTuple):
+    """K and V of several sequences in 8 bits (include/smh.h has the format): blocks of 64 rows with a scale for each kv head, looked up through
+    `pages`; the last block of a sequence in fp16 while it has fewer than 64 rows.  The operators take it, or a tuple of the same tensors."""
+    codes_k: torch.Tensor          # uint8 [pages, Hkv, 64, 128]
+    codes_v: torch.Tensor          # uint8 [pages, Hkv, 128, 64]
+    scales: torch.Tensor           # float32 [pages, Hkv, 2]
+    open_k: torch.Tensor           # fp16 [B, Hkv, 64, 128]
+    open_v: torch.Tensor           # fp16 [B, Hkv, 128, 64]
+    pages: torch.Tensor            # int32 [B, blocks]
+
+
+def kv8_cache(batch: int, max_len: int, n_kv_heads: int, device, n_pages: Optional[int] = None) -> KV8Cache:
+    """An empty cache for `batch` sequences of up to max_len rows.  n_pages None: pages for all of them, block j of sequence b on page
+    b * blocks + j; else that many pages, and a table of -1 (blocks without a page are not written) for the caller to fill in."""
+    assert batch >= 1 and max_len >= 1 and n_kv_heads >= 1 and (n_pages is None or n_pages >= 1)
+    blocks = (max_len + KV8_BLOCK - 1) // KV8_BLOCK
+    n = batch * blocks if n_pages is None else n_pages
+    u8, half = dict(dtype=torch.uint8, device=device), dict(dtype=torch.float16, device=device)
+    if n_pages is None:
+        pages = torch.arange(n, dtype=torch.int32, device=device).view(batch, blocks)
+    else:
+        pages = torch.full((batch, blocks), -1, dtype=torch.int32, device=device)
+    return KV8Cache(torch.full((n, n_kv_heads, KV8_BLOCK, 128), 128, **u8), torch.full((n, n_kv_heads, 128, KV8_BLOCK), 128, **u8),
+                    torch.zeros((n, n_kv_heads, 2), dtype=torch.float32, device=device), torch.zeros((batch, n_kv_heads, KV8_BLOCK, 128), **half),
+                    torch.zeros((batch, n_kv_heads, 128, KV8_BLOCK), **half), pages)
+
+
+def kv8_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, cache, lens: torch.Tensor,
+               cu: Optional[torch.Tensor] = None, max_new: int = 1, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """New rows enter the cache, rotated on the way; returns q rotated, [T, H, 128] fp16.  q [T, H, 128], k and v [T, Hkv, 128] fp16 (views of a packed
+    q|k|v product are fine), cos and sin fp16 [places, 64], lens int32 [B]: rows of each sequence before the call, which stays as it is -
+    the caller adds the new ones to it behind the step's last call.  cu None: one new row a sequence; else int32 [B + 1], sequence b has rows
+    cu[b] .. cu[b + 1] - 1 of the pack, at most max_new.  Rows of no sequence keep what `out` held.  One launch; nothing is read back."""
+    return _lib.ops().kv8_append(q, k, v, cos, sin, cache, lens, cu, max_new, out)
+
+
+def kv8_attn(q: torch.Tensor, cache, lens: torch.Tensor, cu: Optional[torch.Tensor] = None, max_new: int = 1, max_len: Optional[int] = None,
+             window: int = 0, sinks: int = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of the new rows (q as kv8_append returned it, lens as it was given) over the cache that they have entered; [T, H, 128] fp16.
+    window > 0: a query sees its last `window` rows (itself among them) and the first `sinks` of the sequence.  max_len: an upper bound of the longest sequence
+    with its new rows, for the split of the work (default: what the page table holds).  At most two launches; the workspace is the call's own."""
+    return _lib.ops().kv8_attn(q, cache, lens, cu, max_new, max_len, window, sinks, out)
+
+
+def kv8_rows(cache, total: torch.Tensor, first: torch.Tensor, count: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """K and V rows first[b] .. first[b] + count - 1 of every sequence as the cache holds them, fp16 [B, count, Hkv, 128]; rows from total[b] on are 0.
+    total, first: int32 [B]."""
+    return _lib.ops().kv8_rows(cache, total, first, count)
+
+
+# ---------------------------------------------------------------------------------------------
+# beam search
+# ---------------------------------------------------------------------------------------------
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, n: Optional[int] = None, ended: Optional[torch.Tensor] = None, eos: int = 2):
+    """The n (default: beams) best continuations of each group of `beams` rows: (scores float32, parents int32, tokens int64, ended uint8), each [groups, n].
+    logits fp16 [groups * beams, vocab], scores float32 [groups * beams] (log probabilities so far; -inf: no such beam).  Candidates are ordered by
+    score + log_softmax(logits), equal ones by (beam, token); parents are rows within the group.  ended (uint8 or bool, one a row): such a beam goes on as itself,
+    with token eos and its score.  beams <= 64, n <= 128."""
+    return _lib.ops().beam_select(logits, scores, beams, n, ended, eos)
+
+
+def beam_reorder(parents: torch.Tensor, rows: Sequence[torch.Tensor] = (), columns: Sequence[torch.Tensor] = (), upto: Optional[torch.Tensor] = None) -> None:
+    """The states follow the beams, in place: row (g, i) of each tensor [groups * beams, ...] takes the contents of row (g, parents[g, i]).  rows: whole
+    rows (open blocks of a cache, lengths); columns: 2-D int32 or int64 tables of which only the first upto[0] columns (int32 on the device) move (page ids of
+    blocks written so far, tokens so far).  Up to 16 tensors a call, rows a multiple of 4 bytes; one launch."""
+    _lib.ops().beam_reorder(parents, rows, columns, upto)

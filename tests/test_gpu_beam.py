@@ -1,0 +1,221 @@
+"""beam_select and beam_reorder on the GPU against 64 bits and indexing."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+EOS = 2
+
+
+def K():
+    from spec_mcts_amd import kernels
+    return kernels
+
+
+def oracle(logits, scores, W, n, ended=None, eos=EOS):
+    """On the CPU: scores in 64 bits, the n best of each group by (score down, beam, token)"""
+    x, s = logits.double(), scores.double()
+    x = torch.where(torch.isnan(x), torch.full_like(x, -math.inf), x)
+    x = x.clamp(max=65536.0)                                                 # (an infinite logit counts as that)
+    s = torch.where(torch.isnan(s), torch.full_like(s, -math.inf), s)
+    m = x.amax(1, keepdim=True)
+    d = torch.where(x == m, torch.zeros_like(x), x - m)                      # (also where both are infinite)
+    total = s[:, None] + d - torch.log(torch.exp(d).sum(1, keepdim=True))
+    total[(x == -math.inf) | (s == -math.inf)[:, None]] = -math.inf
+    if ended is not None:
+        stay = torch.full_like(total, -math.inf)
+        stay[:, eos] = s
+        total = torch.where(ended.bool()[:, None], stay, total)
+    G, V = logits.shape[0] // W, logits.shape[1]
+    best, at = torch.sort(total.view(G, W * V), dim=1, descending=True, stable=True)
+    best, at = best[:, :n], at[:, :n]
+    parent, token = at // V, at % V
+    done = token == eos
+    if ended is not None:
+        done |= ended.view(G, W).bool().gather(1, parent)
+    return best, parent, token, done
+
+
+def check(logits, scores, W, n, ended=None, eos=EOS):
+    """Whole numbers equal; scores to 2^-22 of the largest term (sums of fp32 exponentials: 2^-23 of the sum each, the result rounded once, 2^-24)"""
+    got = K().beam_select(logits.to(DEV) if not logits.is_cuda else logits, scores.to(DEV), W, n, ended=None if ended is None else ended.to(DEV), eos=eos)
+    best, parent, token, done = oracle(logits.cpu(), scores, W, n, ended, eos)
+    assert torch.equal(got[1].cpu().long(), parent) and torch.equal(got[2].cpu(), token)
+    assert torch.equal(got[3].cpu().bool(), done)
+    s = got[0].cpu().double()
+    fine = torch.isfinite(best)
+    assert torch.equal(s[~fine], best[~fine])
+    assert bool(((s - best)[fine].abs() <= 2.0 ** -22 * (1 + best[fine].abs())).all())
+
+
+def logits_of(rows, vocab, seed, spread=2.0):
+    return (torch.randn((rows, vocab), generator=torch.Generator().manual_seed(seed)) * spread).half()
+
+
+@pytest.mark.parametrize("G,W,n,vocab", [(1, 1, 1, 1), (1, 1, 3, 3), (2, 3, 5, 7), (3, 1, 4, 100), (1, 4, 4, 2047), (2, 4, 8, 2048), (1, 5, 5, 2049), (1, 4, 8, 32016), (2, 64, 128, 300),
+                                         (1, 64, 64, 32016), (70, 8, 16, 2500), (600, 1, 2, 130), (9, 60, 7, 8193), (1, 2, 128, 129280), (130, 4, 4, 8191)])
+@pytest.mark.parametrize("ended", [False, True])
+def test_sizes(G, W, n, vocab, ended):
+    g = torch.Generator().manual_seed(G + W)
+    scores = -torch.rand(G * W, generator=g) * 9
+    done = (torch.rand(G * W, generator=g) < 0.3).to(torch.uint8) if ended else None
+    check(logits_of(G * W, vocab, vocab), scores, W, n, done, eos=min(EOS, vocab - 1))
+
+
+def test_first_step():
+    """all beams are the same prompt and only the first counts; then none does but one"""
+    row = logits_of(1, 32016, 1)
+    scores = torch.full((4,), -math.inf)
+    scores[0] = 0
+    check(row.expand(4, -1).contiguous(), scores, 4, 8)
+    scores[0], scores[2] = -math.inf, math.nan
+    check(row.expand(4, -1).contiguous(), scores, 4, 8)
+    check(row.expand(4, -1).contiguous(), torch.zeros(4), 4, 128)            # equal candidates of all beams
+
+
+@pytest.mark.parametrize("vocab", [50, 2048, 10000])
+@pytest.mark.parametrize("n", [1, 7, 128])
+def test_ties_and_orders(vocab, n):
+    """rows that are all equal, go up, go down, take two values, have their best values next to one another; zeros of both signs"""
+    n = min(n, vocab)
+    i = torch.arange(vocab)
+    rows = [torch.zeros(vocab), i / 16.0, -i / 16.0, (i % 2).float(), torch.where((i >= vocab // 2) & (i < vocab // 2 + 40), 5.0 + i % 3, -i / 999.0), torch.where(i % 2 == 0, 0.0, -0.0),
+            (i % 8 == 7).float() * 3]
+    x = torch.stack(rows).half()
+    for W in (1, 7):
+        check(x, torch.zeros(7), W, n)
+        check(x.flip(0).contiguous(), -torch.arange(7.0), W, n)
+
+
+def test_many_candidates_in_one_thread():
+    """the n largest values stand in as few threads as they can: every slice finds the most keys that it may"""
+    for vocab, threads in ((8192, 128), (2048, 128), (40000, 100)):
+        x = torch.full((1, vocab), -5.0)
+        for t in range(threads):
+            for c in range(vocab // 2048):
+                x[0, c * 2048 + t * 8: c * 2048 + t * 8 + 8] = torch.arange(8) / 8 + t / 4 + c / 64
+        x = x.half()
+        check(x, torch.zeros(1), 1, 128)
+        check(x.expand(600, -1).contiguous()[:, :], torch.zeros(600), 1, 128)        # (in slices of the wide kind)
+
+
+def test_what_is_not_finite():
+    x = logits_of(6, 3000, 5)
+    x[0, :] = -math.inf                                                       # a row that forbids everything
+    x[1, ::2] = math.nan
+    x[2, 100:] = -math.inf
+    x[3, 77] = math.inf
+    x[4, [5, 2500]] = math.inf
+    scores = torch.tensor([0.0, -1.0, -2.0, -0.5, -3.0, -0.25])
+    for W in (1, 2, 3, 6):
+        check(x, scores, W, 20)
+        check(x, scores, W, 20, torch.tensor([0, 1, 0, 0, 0, 1], dtype=torch.uint8))
+    check(torch.full((2, 70), -math.inf).half(), torch.zeros(2), 2, 100 if 100 <= 70 else 70)
+    check(torch.full((2, 70), -math.inf).half(), torch.zeros(2), 2, 70, torch.ones(2, dtype=torch.uint8), eos=69)
+    check(torch.full((2, 70), -math.inf).half(), torch.full((2,), -math.inf), 2, 70, torch.ones(2, dtype=torch.uint8), eos=0)
+
+
+def test_wide_range_of_scores():
+    """sums of scores as long outputs have them, and logits of large magnitude"""
+    check(logits_of(8, 32016, 6, 30.0), -torch.rand(8, generator=torch.Generator().manual_seed(6)) * 4000, 4, 8)
+
+
+def test_strides_and_offsets():
+    """rows further apart than the vocabulary, beginning at any value"""
+    base = logits_of(6, 5003, 7).to(DEV)
+    for a, b in ((0, 5003), (1, 5000), (3, 4100), (8, 2056)):
+        check(base[:, a:b], torch.linspace(-1, 0, 6), 3, 6)
+    check(base.view(-1)[5:5 + 2 * 5003].view(2, 5003), torch.zeros(2), 2, 4)
+
+
+def test_defaults_and_empty():
+    x, s = logits_of(6, 100, 8).to(DEV), torch.zeros(6, device=DEV)
+    a, b = K().beam_select(x, s, 3), K().beam_select(x, s, 3, 3, ended=torch.zeros(6, dtype=torch.bool, device=DEV))
+    assert all(torch.equal(p, q) and p.shape == (2, 3) for p, q in zip(a, b))
+    assert K().beam_select(x[:0], s[:0], 3)[2].shape == (0, 3)
+
+
+def test_captured_and_on_two_streams():
+    x, s = logits_of(8, 32016, 9).to(DEV), torch.linspace(-2, 0, 8, device=DEV)
+    want = [K().beam_select(x.roll(i, 0).contiguous(), s, 4) for i in range(4)]
+    side = torch.cuda.Stream()
+    buf = x.clone()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        K().beam_select(buf, s, 4)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = K().beam_select(buf, s, 4)
+    for i in range(4):
+        buf.copy_(x.roll(i, 0))
+        graph.replay()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            eager = K().beam_select(x, s, 4)
+        assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(eager, want[0]))
+
+
+# ---- reordering -----------------------------------------------------------------------------------------------------------------
+def moved(x, parents, cols=None):
+    G, W = parents.shape
+    row = (torch.arange(G, device=x.device)[:, None] * W + parents.to(x.device).clamp(0, W - 1)).view(-1)
+    y = x.clone()
+    if cols is None:
+        y[:] = x[row]
+    else:
+        y[:, :cols] = x[row][:, :cols]
+    return y
+
+
+@pytest.mark.parametrize("G,W", [(1, 1), (1, 2), (3, 4), (2, 64), (17, 5)])
+@pytest.mark.parametrize("upto", [0, 1, 33, 1000, 2 ** 31 - 1, -5])
+def test_states_follow(G, W, upto):
+    g = torch.Generator(device=DEV).manual_seed(G * W)
+    R = G * W
+    cols = [torch.randint(0, 1 << 30, (R, 133), device=DEV, generator=g).int(), torch.randint(0, 1 << 60, (R, 50), device=DEV, generator=g)]
+    rows = [torch.randn((R, 2, 64, 128), device=DEV, generator=g).half(), torch.randn(R, device=DEV, generator=g), torch.randn((R, 7, 3), device=DEV, generator=g),
+            torch.randint(0, 255, (R, 64), device=DEV, generator=g).to(torch.uint8)]
+    for parents in (torch.arange(W).repeat(G, 1), torch.arange(W).roll(1).repeat(G, 1), torch.zeros((G, W)), torch.randint(0, W, (G, W), generator=torch.Generator().manual_seed(W)),
+                    torch.randint(-3, W + 3, (G, W), generator=torch.Generator().manual_seed(W))):
+        parents = parents.to(torch.int32).to(DEV)
+        want = [moved(x, parents) for x in rows] + [moved(x, parents, min(max(upto, 0), x.shape[1])) for x in cols]
+        K().beam_reorder(parents, rows=rows, columns=cols, upto=torch.tensor([upto], dtype=torch.int32, device=DEV))
+        assert all(torch.equal(a, b) for a, b in zip(rows + cols, want))
+
+
+def test_strided_and_odd_states():
+    """rows of a wider tensor (what lies between them stays), widths that are no multiple of 16 bytes, empty ones, none at all"""
+    wide = torch.arange(12 * 100, device=DEV, dtype=torch.int32).view(12, 100).clone()
+    parents = torch.tensor([[3, 0, 0, 1], [1, 1, 2, 0], [0, 1, 2, 3]], dtype=torch.int32, device=DEV)
+    want = wide.clone()
+    want[:, 10:47] = moved(wide[:, 10:47], parents)
+    K().beam_reorder(parents, rows=[wide[:, 10:47], torch.empty((12, 0), device=DEV)])
+    assert torch.equal(wide, want)
+    want[:, 1:90] = moved(wide[:, 1:90], parents, 60)
+    K().beam_reorder(parents, columns=[wide[:, 1:90]], upto=torch.tensor([60], dtype=torch.int32, device=DEV))
+    assert torch.equal(wide, want)
+    K().beam_reorder(parents)
+    K().beam_reorder(parents[:0], rows=[wide[:0]])
+
+
+def test_captured_reorder():
+    x = torch.randn((8, 4, 64, 128), device=DEV).half()
+    t = torch.arange(8 * 40, device=DEV, dtype=torch.int32).view(8, 40).clone()
+    parents, n = torch.zeros((2, 4), dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    K().beam_reorder(parents + torch.arange(4, dtype=torch.int32, device=DEV), rows=[x], columns=[t], upto=n)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        K().beam_reorder(parents, rows=[x], columns=[t], upto=n)
+    for i, p in enumerate(([[1, 0, 3, 2], [0, 0, 0, 0]], [[3, 3, 1, 0], [2, 1, 0, 3]], [[0, 1, 2, 3], [1, 2, 3, 0]])):
+        parents.copy_(torch.tensor(p, dtype=torch.int32))
+        n.fill_(10 * i + 5)
+        want = moved(x, parents), moved(t, parents, 10 * i + 5)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(x, want[0]) and torch.equal(t, want[1])

@@ -1,0 +1,423 @@
+"""The paged 8-bit cache on the GPU against tests/kv8_oracle.py: what enters it bit for bit, attention against 64 bits."""
+import math
+import random
+
+import pytest
+import torch
+
+from tests import kv8_oracle as O
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def K():
+    from spec_mcts_amd import kernels
+    return kernels
+
+
+class World:
+    """A cache on the GPU and the same sequences in the oracle"""
+
+    def __init__(self, B, H, Hkv, max_len, seed, spare=3, places=None, scale=1.0):
+        self.g = torch.Generator().manual_seed(seed)
+        self.B, self.H, self.Hkv = B, H, Hkv
+        self.cols = (max_len + 63) // 64
+        n = B * self.cols + spare
+        self.cache = K().kv8_cache(B, max_len, Hkv, DEV, n_pages=n)
+        order = torch.randperm(n, generator=self.g)[:B * self.cols].view(B, self.cols).to(torch.int32)
+        self.cache.pages.copy_(order)
+        self.cache.open_k.fill_(math.nan)                       # what no row was written to may hold anything
+        self.cache.open_v.fill_(math.nan)
+        self.cache.scales.fill_(math.nan)
+        self.cos, self.sin = O.tables(places or max_len + 64)
+        self.cos_d, self.sin_d = self.cos.to(DEV), self.sin.to(DEV)
+        self.seqs = [O.Sequence(Hkv) for _ in range(B)]
+        self.lens = torch.zeros(B, dtype=torch.int32, device=DEV)
+        self.scale = scale
+
+    def old(self):
+        return [s.k.shape[0] for s in self.seqs]
+
+    def rows(self, T):
+        r = lambda h, s: (torch.randn((T, h, 128), generator=self.g) * s).half()
+        return r(self.H, 1.5), r(self.Hkv, 1.5 * self.scale), r(self.Hkv, self.scale)
+
+    def step(self, new, qkv=None, behind=0, advance=True, max_new=None, single=False, packed=False):
+        """`new` rows for each sequence; (q rotated on the GPU, q rotated by the oracle, cu)"""
+        T = sum(new) + behind
+        q, k, v = qkv or self.rows(T)
+        cu = None if single else torch.tensor([sum(new[:b]) for b in range(self.B + 1)], dtype=torch.int32, device=DEV)
+        if packed:
+            p = torch.cat([x.reshape(T, -1) for x in (q, k, v)], 1).to(DEV)
+            a, b = self.H * 128, (self.H + self.Hkv) * 128
+            args = p[:, :a].view(T, self.H, 128), p[:, a:b].view(T, self.Hkv, 128), p[:, b:].view(T, self.Hkv, 128)
+        else:
+            args = q.to(DEV), k.to(DEV), v.to(DEV)
+        out = torch.full((T, self.H, 128), 7.0, dtype=torch.float16, device=DEV)
+        got = K().kv8_append(*args, self.cos_d, self.sin_d, self.cache, self.lens, cu=cu, max_new=1 if single else max_new or max(max(new), 1), out=out)
+        assert got is out
+        want = torch.full((T, self.H, 128), 7.0, dtype=torch.float16)
+        at = 0
+        for s, n in zip(self.seqs, new):
+            place = torch.arange(s.k.shape[0], s.k.shape[0] + n).clamp(max=self.cos.shape[0] - 1)
+            want[at:at + n] = O.rotate(q[at:at + n], self.cos, self.sin, place)
+            s.add(O.rotate(k[at:at + n], self.cos, self.sin, place), v[at:at + n])
+            at += n
+        self.before = self.lens.clone()
+        if advance:
+            self.lens += torch.tensor(new, dtype=torch.int32, device=DEV)
+        return got, want, cu
+
+    def check_cache(self):
+        """codes and scales of whole blocks and the rows of open ones, bit for bit"""
+        c = [t.cpu() for t in self.cache]
+        for b, s in enumerate(self.seqs):
+            n = s.k.shape[0]
+            for j in range(min(n // 64, self.cols)):
+                page = int(c[5][b, j])
+                codes, scales = s.block(j)
+                assert torch.equal(c[0][page], codes[0]), (b, j)
+                assert torch.equal(c[1][page], codes[1].transpose(1, 2)[..., torch.argsort(torch.tensor(O.PLACE))]), (b, j)
+                assert torch.equal(c[2][page], torch.stack(scales, -1)), (b, j)
+            left = n % 64
+            assert torch.equal(c[3][b, :, :left], s.k[n - left:].transpose(0, 1)), b
+            assert torch.equal(c[4][b][..., O.PLACE[:left]], s.v[n - left:].permute(1, 2, 0)), b
+
+    def check_attn(self, q, new, cu, **kw):
+        """q: as kv8_append returned it, behind the step that brought `new`"""
+        window, sinks = kw.get("window", 0), kw.get("sinks", 0)
+        out = torch.full(q.shape, 9.0, dtype=torch.float16, device=DEV)
+        got = K().kv8_attn(q, self.cache, self.before, cu=cu, max_new=max(max(new), 1), out=out, **kw)
+        assert got is out
+        got, q = got.cpu().double(), q.cpu()
+        at = 0
+        for b, (s, n) in enumerate(zip(self.seqs, new)):
+            k, v = s.held()
+            old = k.shape[0] - n
+            o, mean = O.attention(q[at:at + n], k, v, old, window, sinks)
+            bound = O.attention_bound(o, mean, k.shape[0], float(v.abs().max()) if v.numel() else 0.0)
+            off = (got[at:at + n] - o).abs()
+            assert bool((off <= bound).all()), (b, old, n, float((off / bound).max()))
+            at += n
+        assert bool((got[at:] == 9.0).all())                    # rows behind the last sequence
+
+
+# ---- what enters the cache -----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("B,H,Hkv", [(1, 1, 1), (3, 4, 4), (2, 8, 1), (5, 12, 4), (2, 40, 2)])
+def test_single_tokens_across_blocks(B, H, Hkv):
+    """one row at a time from an empty cache past two borders of a block"""
+    w = World(B, H, Hkv, 200, seed=B * 100 + H)
+    for i in range(131):
+        got, want, _ = w.step([1] * B, single=i % 2 == 0, packed=i % 3 == 0)
+        assert torch.equal(got.cpu(), want), i
+        if i in (0, 62, 63, 64, 130):
+            w.check_cache()
+
+
+@pytest.mark.parametrize("steps", [[[1, 2, 3]], [[63, 64, 65], [1, 1, 1]], [[63, 1, 62], [2, 0, 5], [0, 0, 0], [130, 64, 1]], [[200, 7, 0], [57, 121, 300], [1, 1, 1], [63, 64, 65]],
+                                   [[127, 128, 129], [129, 128, 127], [65, 64, 63]], [[1, 0, 500]]], ids=str)
+def test_ragged_packs(steps):
+    w = World(3, 6, 2, 700, seed=len(steps))
+    for i, new in enumerate(steps):
+        got, want, _ = w.step(new, behind=i, packed=i % 2 == 1)
+        assert torch.equal(got.cpu(), want), i                  # (the rows behind the last sequence among them)
+        w.check_cache()
+
+
+def test_what_it_holds_does_not_depend_on_the_calls():
+    """the same 300 rows in one call, in chunks and row by row: the same bytes"""
+    rng = random.Random(3)
+    seen = []
+    for way in ("one", "chunks", "rows"):
+        w = World(2, 4, 2, 320, seed=11)
+        q, k, v = w.rows(600)
+        at = 0
+        while at < 300:
+            n = 300 if way == "one" else 1 if way == "rows" else min(rng.randint(1, 140), 300 - at)
+            pick = torch.cat((torch.arange(at, at + n), torch.arange(300 + at, 300 + at + n)))
+            w.step([n, n], qkv=(q[pick], k[pick], v[pick]))
+            at += n
+        w.check_cache()
+        seen.append([t[w.cache.pages.long()].cpu()[:, :4] for t in w.cache[:3]])
+    assert all(torch.equal(a, b) for other in seen[1:] for a, b in zip(seen[0], other))
+
+
+def test_bad_pages_and_lengths_write_nothing():
+    """a block without a page, past the table or past the capacity is not written, and nothing else is touched"""
+    w = World(4, 2, 2, 128, seed=5)
+    n_pages = w.cache.codes_k.shape[0]
+    w.cache.pages[0, 0] = -1
+    w.cache.pages[1, 0] = n_pages
+    w.cache.pages[1, 1] = 2 ** 31 - 1
+    before = [t.clone() for t in w.cache]
+    lens = torch.tensor([0, 0, 128, 2 ** 31 - 1], dtype=torch.int32, device=DEV)
+    T = 4 * 130
+    q, k, v = (x.to(DEV) for x in w.rows(T))
+    cu = torch.arange(0, T + 1, 130, dtype=torch.int32, device=DEV)
+    K().kv8_append(q, k, v, w.cos_d, w.sin_d, w.cache, lens, cu=cu, max_new=130)
+    kept = {int(w.cache.pages[0, 1])}                           # the one block that has a page and a place
+    for t, old in zip(w.cache[:3], before[:3]):
+        changed = {p for p in range(n_pages) if not torch.equal(t[p].cpu().view(torch.uint8), old[p].cpu().view(torch.uint8))}
+        assert changed <= kept
+    assert int((w.cache.scales[list(kept)] > 0).sum()) == 4
+    for t, old in zip(w.cache[3:5], before[3:5]):
+        assert torch.equal(t[2:].view(torch.int16), old[2:].view(torch.int16))      # sequences whose rows end past the capacity
+
+
+def test_numbers_past_the_tensors_are_cut():
+    """cu past the pack or going down, negative lengths, max_new below what cu says"""
+    w = World(3, 2, 1, 64, seed=6)
+    q, k, v = (x.to(DEV) for x in w.rows(10))
+    for cu, lens in (([0, 4, 99, 100], [0, 0, 0]), ([0, 8, 3, 10], [0, -5, 0]), ([-7, 2, 4, 9], [-1, 0, 3])):
+        out = torch.full_like(q, 7.0)
+        K().kv8_append(q, k, v, w.cos_d, w.sin_d, w.cache, torch.tensor(lens, dtype=torch.int32, device=DEV), cu=torch.tensor(cu, dtype=torch.int32, device=DEV), max_new=3, out=out)
+        o = K().kv8_attn(out, w.cache, torch.tensor(lens, dtype=torch.int32, device=DEV), cu=torch.tensor(cu, dtype=torch.int32, device=DEV), max_new=3)
+        a = min(max(cu[0], 0), 10)
+        assert torch.equal(out[a:a + 2].cpu(), O.rotate(q[a:a + 2].cpu(), w.cos, w.sin, torch.arange(2) + max(lens[0], 0)))
+        assert torch.isfinite(o[a:a + 2]).all()
+
+
+def test_places_past_the_tables_take_the_last_row():
+    w = World(2, 2, 2, 256, seed=7, places=70)
+    got, want, _ = w.step([100, 69])
+    assert torch.equal(got.cpu(), want)
+    got, want, _ = w.step([1, 1], single=True)
+    assert torch.equal(got.cpu(), want)
+    w.check_cache()
+
+
+def test_zeros_and_extremes():
+    """blocks of zeros have a scale of 0; the largest and the least fp16 values keep their block's codes in 1 .. 255"""
+    w = World(2, 2, 2, 128, seed=8)
+    q, k, v = w.rows(256)
+    k[:64], v[:64] = 0, 0
+    v[64:128] = 65504.0
+    k[128:192] = 2.0 ** -24
+    v[128:192] *= 2.0 ** -20
+    w.step([128, 128], qkv=(q, k, v))
+    w.check_cache()
+    assert int(w.cache.codes_k[w.cache.pages.long()].min()) >= 1
+    rows = K().kv8_rows(w.cache, w.lens, torch.zeros_like(w.lens), 128)
+    assert bool((rows[0][0, :64] == 0).all()) and bool((rows[1][0, 64:128] == 65504.0).all())
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_what_is_not_finite_stays_in_its_block_and_head(bad):
+    w = World(1, 2, 2, 256, seed=9)
+    q, k, v = w.rows(200)
+    v[70, 0, 5] = bad
+    k2 = k.clone()
+    w.step([200], qkv=(q, k2, v), advance=True)
+    rows_k, rows_v = K().kv8_rows(w.cache, w.lens, torch.zeros_like(w.lens), 200)
+    assert bool(torch.isfinite(rows_k).all())
+    fine = torch.ones((200, 2), dtype=torch.bool)
+    fine[64:128, 0] = False
+    assert torch.equal(torch.isfinite(rows_v[0]).all(-1).cpu(), fine) and bool(torch.isnan(rows_v[0, 64:128, 0]).all())
+    # attention: head 1 and the queries in front of the block are as they were
+    cu = torch.tensor([0, 200], dtype=torch.int32, device=DEV)
+    o = K().kv8_attn(q.to(DEV), w.cache, w.before, cu=cu, max_new=200)[:, :, :].cpu()
+    assert bool(torch.isfinite(o[:, 1]).all()) and bool(torch.isfinite(o[:64, 0]).all()) and bool(torch.isnan(o[64:, 0]).all())
+
+
+@pytest.mark.parametrize("first,count", [([0, 0, 0], 1), ([0, 63, 64], 66), ([5, 130, 199], 130), ([0, 0, 0], 300), ([1000, -4, 150], 64), ([0, 1, 2], 0)], ids=str)
+def test_rows_come_back(first, count):
+    w = World(3, 2, 2, 256, seed=10)
+    w.step([200, 131, 64])
+    f = torch.tensor(first, dtype=torch.int32, device=DEV)
+    k, v = K().kv8_rows(w.cache, w.lens, f, count)
+    assert k.shape == v.shape == (3, count, 2, 128)
+    for b, s in enumerate(w.seqs):
+        for got, x in zip((k, v), s.held()):
+            want = torch.zeros((count, 2, 128), dtype=torch.float64)
+            a = max(first[b], 0)
+            part = x[a:a + count]
+            want[:part.shape[0]] = part
+            assert torch.equal(got[b].cpu(), want.float().half()), b      # (a code times its scale: fp32 rounds once before fp16)
+
+
+# ---- attention -------------------------------------------------------------------------------------------------------------------
+SIGHTS = [(0, 0), (1, 0), (5, 3), (64, 0), (64, 64), (100, 4), (200, 130), (4096, 4), (37, 4096)]
+
+
+@pytest.mark.parametrize("window,sinks", SIGHTS, ids=str)
+@pytest.mark.parametrize("H,Hkv", [(1, 1), (4, 4), (8, 1), (6, 2), (32, 2)])
+def test_one_query(H, Hkv, window, sinks):
+    """one token for sequences of length 0 to 1000, no two alike"""
+    old = [0, 1, 62, 63, 64, 65, 127, 300, 511, 999]
+    w = World(len(old), H, Hkv, 1024, seed=H * 1000 + window + sinks)
+    w.step(old)
+    q, _, cu = w.step([1] * len(old), single=True)
+    w.check_attn(q, [1] * len(old), cu, window=window, sinks=sinks)
+    w.check_attn(q, [1] * len(old), cu, window=window, sinks=sinks, max_len=1000)
+
+
+@pytest.mark.parametrize("window,sinks", SIGHTS, ids=str)
+@pytest.mark.parametrize("H,Hkv,new", [(4, 4, [3, 0, 7, 5]), (8, 1, [2, 1, 2, 0]), (8, 1, [4, 3, 4, 1]), (8, 1, [6, 5, 0, 6]), (8, 1, [8, 8, 1, 3]), (6, 2, [17, 21, 2, 9])])
+def test_a_few_queries(H, Hkv, new, window, sinks):
+    """all tile counts of the kernel for up to 64 queries a head"""
+    w = World(4, H, Hkv, 1024, seed=H + sum(new) + window)
+    w.step([500, 61, 0, 190])
+    q, _, cu = w.step(new, behind=2)
+    w.check_attn(q, new, cu, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("window,sinks", SIGHTS, ids=str)
+@pytest.mark.parametrize("H,Hkv,old,new", [(2, 2, [0, 0], [130, 65]), (8, 1, [64, 333], [40, 9]), (6, 2, [700, 5], [100, 250]), (4, 4, [1, 0], [0, 300]), (16, 1, [100, 640], [64, 63])])
+def test_many_queries(H, Hkv, old, new, window, sinks):
+    w = World(2, H, Hkv, 1024, seed=H + sum(new) + window)
+    w.step(old)
+    q, _, cu = w.step(new, behind=3)
+    w.check_attn(q, new, cu, window=window, sinks=sinks)
+    w.check_attn(q, new, cu, window=window, sinks=sinks, max_len=sum(new) + max(old))
+
+
+@pytest.mark.parametrize("max_len", [1, 64, 5000, 10 ** 6])
+@pytest.mark.parametrize("new", [[1], [30], [200]])
+def test_every_split_of_a_long_sequence(max_len, new):
+    """max_len decides the split alone: also one that is too small gives the same attention"""
+    w = World(1, 2, 1, 5000, seed=len(new) + max_len)
+    w.step([4700])
+    q, _, cu = w.step(new)
+    w.check_attn(q, new, cu, max_len=max_len)
+    w.check_attn(q, new, cu, max_len=max_len, window=1500, sinks=70)
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -12, 2.0 ** -6, 64.0])
+def test_small_and_large_values(scale):
+    """V of all sizes next to an open block: scales meet in fp32"""
+    w = World(2, 4, 2, 512, seed=21, scale=scale)
+    if scale > 1:
+        q, k, v = w.rows(400)
+        w.step([200, 200], qkv=(q, k / 64, v))                 # (scores stay below 64)
+        q, k, v = w.rows(2)
+        q, _, cu = w.step([1, 1], qkv=(q, k / 64, v))
+    else:
+        w.step([200, 200])
+        q, _, cu = w.step([1, 1])
+    w.check_attn(q, [1, 1], cu)
+
+
+def test_steep_scores():
+    """a maximum that grows block by block, and one that stands in the first row"""
+    for order in (1, -1):
+        w = World(1, 2, 1, 1024, seed=22)
+        q, k, v = w.rows(701)
+        q[:] = 0
+        q[..., 0] = 1.0
+        k[:] = 0
+        k[:, :, 0] = (200 + order * torch.linspace(-200, 200, 701))[:, None].half()
+        w.cos_d.fill_(1), w.sin_d.fill_(0)
+        w.cos.fill_(1), w.sin.fill_(0)
+        w.step([700], qkv=(q[:700], k[:700], v[:700]))
+        got, _, cu = w.step([1], qkv=(q[700:], k[700:], v[700:]))
+        w.check_attn(got, [1], cu)
+
+
+def test_pages_out_of_range_are_read_as_the_nearest():
+    w = World(2, 2, 2, 256, seed=23)
+    w.step([256, 256])
+    w.cache.scales.nan_to_num_(0.01)
+    w.cache.pages[0, 1] = -9
+    w.cache.pages[1, 2] = 10 ** 6
+    q, _, _ = w.rows(2)
+    w.before = w.lens - 1
+    ref = w.cache.pages.clamp(0, w.cache.codes_k.shape[0] - 1)
+    got = K().kv8_attn(q.to(DEV), w.cache, w.before, max_len=256)
+    assert torch.equal(got, K().kv8_attn(q.to(DEV), w.cache._replace(pages=ref), w.before, max_len=256))
+
+
+def test_tables_wider_than_the_batch_and_strided_queries():
+    """a slice of a wider page table, a smaller batch than the cache's, queries out of a packed product"""
+    w = World(4, 4, 2, 512, seed=24)
+    w.step([300, 10, 64, 200])
+    wide = torch.full((4, w.cols + 5), -1, dtype=torch.int32, device=DEV)
+    wide[:, 2:2 + w.cols] = w.cache.pages
+    q, _, cu = w.step([1, 1, 1, 1], packed=True)
+    packed = torch.randn((4, 8, 128), device=DEV).half()
+    packed[:, 4:] = q
+    one = K().kv8_attn(q, w.cache, w.before)
+    part = K().kv8_attn(packed[:2, 4:], w.cache._replace(pages=wide[:, 2:2 + w.cols]), w.before[:2])
+    assert torch.equal(part, one[:2])
+    assert K().kv8_attn(q[:0], w.cache, w.before[:0]).shape == (0, 4, 128)
+    w.check_attn(q, [1] * 4, cu)
+
+
+def test_a_nan_query_has_a_nan_output():
+    w = World(1, 2, 1, 4096, seed=25)
+    w.step([3000])
+    q, _, cu = w.step([1])
+    q[0, 1] = math.nan
+    for max_len in (64, 4096):
+        o = K().kv8_attn(q, w.cache, w.before, max_len=max_len).cpu()
+        assert bool(torch.isnan(o[0, 1]).all()) and bool(torch.isfinite(o[0, 0]).all())
+
+
+def test_captured_steps():
+    """one graph of append, attention and the step of the lengths, replayed over a border of a block with eager work between, against eager steps"""
+    worlds = [World(3, 4, 2, 512, seed=26) for _ in range(2)]
+    for w in worlds:
+        w.step([60, 126, 300])
+    rows = [worlds[0].rows(3) for _ in range(6)]
+    eager, graphed = worlds
+    want = []
+    for r in rows:
+        q, _, cu = eager.step([1, 1, 1], qkv=r, single=True)
+        want.append(K().kv8_attn(q, eager.cache, eager.before, max_len=512).clone())
+    q, k, v = (x.to(DEV) for x in rows[0])
+    lens, one = graphed.lens, torch.ones(3, dtype=torch.int32, device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):                               # warm up
+        K().kv8_attn(K().kv8_append(q, k, v, graphed.cos_d, graphed.sin_d, graphed.cache, lens), graphed.cache, lens, max_len=512)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        rotated = K().kv8_append(q, k, v, graphed.cos_d, graphed.sin_d, graphed.cache, lens)
+        out = K().kv8_attn(rotated, graphed.cache, lens, max_len=512)
+        lens += one
+    for r, o in zip(rows, want):
+        for t, x in zip((q, k, v), r):
+            t.copy_(x)
+        graph.replay()
+        assert torch.equal(out, o)
+        torch.randn((64, 64), device=DEV).sum()
+        torch.cuda.synchronize()
+    for a, b in zip(eager.cache[:3], graphed.cache[:3]):
+        assert torch.equal(a[eager.cache.pages[:, 0].long()], b[graphed.cache.pages[:, 0].long()])
+
+
+def test_two_streams_at_once():
+    """attention over one cache from two streams, split and merged: each call has its own workspace"""
+    w = World(1, 2, 1, 8192, seed=27)
+    w.step([8000])
+    q, _, cu = w.step([1])
+    other = q.flip(1).contiguous()
+    want = [K().kv8_attn(x, w.cache, w.before, max_len=8192) for x in (q, other)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        for i, x in enumerate((q, other)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(K().kv8_attn(x, w.cache, w.before, max_len=8192))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i]) for i in range(2) for o in got[i])
+
+
+def test_offsets_past_32_bits():
+    """pages whose codes lie more than 4 GiB into the pool"""
+    Hkv, n_pages = 8, 70000                                     # 70000 x 8 x 8 KiB = 4.6 GB a side
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    c = K().kv8_cache(1, 256, Hkv, DEV, n_pages=n_pages)
+    w = World(1, 8, Hkv, 256, seed=28)
+    w.cache = c
+    c.pages.copy_(torch.tensor([[69999, 3, 69000, 65536]], dtype=torch.int32))
+    w.step([250])
+    q, _, cu = w.step([1])
+    w.check_cache()
+    w.check_attn(q, [1], cu)
+    k, _ = K().kv8_rows(c, w.lens, torch.zeros_like(w.lens), 251)
+    assert torch.equal(k[0].cpu(), w.seqs[0].held()[0].float().half())
