@@ -3,8 +3,8 @@
 // Selection.  Candidate (beam r, token t) of a group has the score  scores[r] + x[r][t] - log sum_t' exp(x[r][t']);  the n best leave in descending order,
 // equal ones by (beam, token).  A first launch goes over each row once, a workgroup per slice of it: the slice's values stay in registers while its maximum, its sum of
 // exponentials and its n largest values are found.  A second one has a wave per group: it adds the slices' sums up and merges their sorted lists.
-//   Order: within a row the fp16 values order exactly; between rows the scores are compared in 64 bits, with sums whose terms are fp32 (2^-23 each, the sum of a
-//   slice in 64 bits), so that candidates keep their order unless they are closer than that.
+//   Order: within a row the fp16 values order exactly; between rows the scores are compared in 64 bits, with sums in 64 bits of fp32 terms, so that
+//   candidates keep their order unless they are closer than the terms' roundings (2^-24 each) leave the sums.
 // Bound: HBM, 2 bytes a logit; the smallest calls by the two launches.
 //
 // Reordering.  Row i of a group takes the contents of row parents[i], in place: a workgroup owns a strip of all rows of a group, has it in LDS and then writes.
@@ -20,7 +20,7 @@ struct SelectParams {
     long ld;
     const float *scores;
     const uint8_t *ended;                          // may be null
-    int rows, W, G, vocab, n, eos, slices, width;  // width: columns of a slice
+    int rows, W, G, vocab, n, eos, slices, width, held;      // width: columns of a slice; held: the second launch has all lists in LDS
     float *slice_max;                              // [rows][slices]
     double *slice_sum;                             // [rows][slices], of exp(x - slice_max)
     uint32_t *cand;                                // [rows][slices][n]: keys (below), descending; 0: none
@@ -32,83 +32,56 @@ struct SelectParams {
 
 // A value's key: 16 bits that order as the values do (NaN as the least), then 16 bits that are larger for earlier columns of the slice: keys of a slice differ.
 __device__ __forceinline__ uint32_t beam_order(half_t x) {
-    uint32_t b = __builtin_bit_cast(uint16_t, x);
-    if ((b & 0x7FFFu) > 0x7C00u) b = 0xFC00u;      // NaN: -infinity
-    if (b == 0x8000u) b = 0;                       // -0 is 0
+    const uint32_t b = __builtin_bit_cast(uint16_t, x);
     return b & 0x8000u ? 0xFFFFu - b : b | 0x8000u;
 }
 __device__ __forceinline__ float beam_value(uint32_t order) {
     const uint32_t b = order & 0x8000u ? order & 0x7FFFu : 0xFFFFu - order;
     return fminf((float)__builtin_bit_cast(half_t, (uint16_t)b), 65536.0f);      // (an infinity is the step after 65504: the others of its row stay in order)
 }
-__device__ __forceinline__ uint32_t beam_key(half_t x, int col) { return beam_order(x) << 16 | (0xFFFFu - (uint32_t)col); }
 
-// exp(x), x <= 0, with the rounding of x log2(e) made good: about 2^-23
-__device__ __forceinline__ float beam_exp(float x) {
-    if (x < -104.0f) return 0.0f;                  // (below the least float; x may be -infinity)
-    const float hi = x * 1.44269504f, lo = __builtin_fmaf(x, 1.44269504f, -hi) + x * 1.92596299e-8f;
-    const float e = __builtin_amdgcn_exp2f(hi);
-    return __builtin_fmaf(e * 0.693147181f, lo, e);
-}
-
-// 256 threads, VPT values each: a slice of 256 * VPT columns.
-template <int VPT>
+// 256 threads, CHUNKS * 8 values each, chunk i of thread t being columns (256 i + t) * 8 .. + 7: a slice of 2048 * CHUNKS columns.
+template <int CHUNKS>
 __global__ __launch_bounds__(256) void beam_slice_kernel(SelectParams p) {
-    constexpr int CHUNKS = VPT / 8;
-    __shared__ uint32_t top[256];                  // each thread's largest key
-    __shared__ uint32_t found[VPT * BEAM_MAX_N];   // keys not below the n-th of them: at most VPT of each of n threads
-    __shared__ uint32_t red_max[4];
+    __shared__ uint32_t top[256];                  // each thread's largest value and the first of its chunks that has it
+    extern __shared__ uint32_t found[];            // candidates: at most all values of n threads
     __shared__ double red_sum[4];
     __shared__ int n_found;
     const int slice = blockIdx.x, row = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int c0 = slice * p.width, cols = min(p.width, p.vocab - c0), n = p.n;
     uint32_t *cand = p.cand + ((long)row * p.slices + slice) * n;
-    const float score = p.scores[row];
-    const bool ended = p.ended != nullptr && p.ended[row] != 0, lost = !(score > -INFINITY);
-    if (ended || lost) {
-        // No value counts: a lost beam's candidates are all -infinity and go by their index; of an ended beam's the first is its end, the others go by index
-        // too (which the second launch does, too)
-        return;
-    }
+    // No value of a lost or ended beam counts: its candidates go by their index, which the second launch does by itself
+    if (!(p.scores[row] > -INFINITY) || (p.ended != nullptr && p.ended[row] != 0)) return;
     const half_t *x = p.logits + (long)row * p.ld + c0;
-    uint32_t key[VPT];
-    uint32_t mine = 0;
+    const h8 least = {-(half_t)INFINITY, -(half_t)INFINITY, -(half_t)INFINITY, -(half_t)INFINITY, -(half_t)INFINITY, -(half_t)INFINITY, -(half_t)INFINITY, -(half_t)INFINITY};
+    h8 v[CHUNKS];
     const bool aligned = ((uintptr_t)x & 15) == 0;
 #pragma unroll
     for (int i = 0; i < CHUNKS; ++i) {
         const int col = (i * 256 + t) * 8;
-        h8 v;
-        if (aligned && col + 8 <= cols) v = *reinterpret_cast<const h8 *>(x + col);
+        if (aligned && col + 8 <= cols) v[i] = *reinterpret_cast<const h8 *>(x + col);
         else {
+            v[i] = least;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = col + e < cols ? x[col + e] : (half_t)0.0f;
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            key[i * 8 + e] = col + e < cols ? beam_key(v[e], col + e) : 0u;
-            mine = max(mine, key[i * 8 + e]);
+            for (int e = 0; e < 8; ++e)
+                if (col + e < cols) v[i][e] = x[col + e];
         }
     }
-    top[t] = mine;
-    uint32_t most = mine;
+    // the thread's key: order of its largest value, then the chunks' order (they are in the columns' order), 0 without columns
+    uint32_t mine = 0;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, o, 64));
-    if (lane == 0) red_max[wave] = most;
+    for (int i = 0; i < CHUNKS; ++i) {
+        v[i] = __builtin_elementwise_max(v[i], least);                 // (NaN: -infinity)
+        const h4 a = __builtin_elementwise_max(__builtin_shufflevector(v[i], v[i], 0, 1, 2, 3), __builtin_shufflevector(v[i], v[i], 4, 5, 6, 7));
+        const h2 b = __builtin_elementwise_max(__builtin_shufflevector(a, a, 0, 1), __builtin_shufflevector(a, a, 2, 3));
+        const half_t m = __builtin_elementwise_max(b[0], b[1]) + (half_t)0.0f;      // (+ 0: one zero)
+        const uint32_t key = beam_order(m) << 16 | (0xFFFFu - (uint32_t)(i * 256 + t));
+        if ((i * 256 + t) * 8 < cols) mine = max(mine, key);
+    }
+    top[t] = mine;
     if (t == 0) n_found = 0;
     __syncthreads();
-    const float m = beam_value(max(max(red_max[0], red_max[1]), max(red_max[2], red_max[3])) >> 16);      // (every slice has a column)
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < VPT; ++i)
-        if (key[i] != 0) {
-            const float v = beam_value(key[i] >> 16);
-            sum += v == m ? 1.0f : beam_exp(v - m);                    // (v == m: also both -infinity)
-        }
-    double total = sum;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
-    if (lane == 0) red_sum[wave] = total;
-    // the n-th largest of the threads' largest keys, bit by bit: n keys are not below it, and no key below it is among the n largest
+    // The n-th largest of these keys, bit by bit.  n threads are not below it; a value that is, by (value, chunk), has n better ones.
     uint32_t mx[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) mx[i] = top[i * 64 + lane];
@@ -121,9 +94,32 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(SelectParams p) {
         for (int i = 0; i < 4; ++i) c += __popcll(__ballot(mx[i] >= at));
         if (c >= n) bar = at;
     }
+    if (mine >= bar && mine != 0) {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i)
-        if (key[i] >= bar && key[i] != 0) found[atomicAdd(&n_found, 1)] = key[i];
+        for (int i = 0; i < CHUNKS; ++i) {
+            const uint32_t chunk = i * 256 + t;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t order = beam_order(v[i][e] + (half_t)0.0f);
+                if ((order << 16 | (0xFFFFu - chunk)) >= bar && (int)(chunk * 8 + e) < cols) found[atomicAdd(&n_found, 1)] = order << 16 | (0xFFFFu - (chunk * 8 + e));
+            }
+        }
+    }
+    uint32_t most = max(max(mx[0], mx[1]), max(mx[2], mx[3]));
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, o, 64));
+    const float m = beam_value(most >> 16);                            // (every slice has a column)
+    // exp(x - m): the difference is exact or rounded once, its product with log2(e) is off by 2^-24 of itself, so terms near the largest have 2^-23
+    double total = 0.0;
+    if (m > -INFINITY) {
+#pragma unroll
+        for (int i = 0; i < CHUNKS; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) total += (double)__builtin_amdgcn_exp2f((fminf((float)v[i][e], 65536.0f) - m) * 1.44269504f);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
+    if (lane == 0) red_sum[wave] = total;
     __syncthreads();
     const int have = n_found;
     if (t == 0) {
@@ -140,90 +136,102 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(SelectParams p) {
     for (int i = have + t; i < n; i += 256) cand[i] = 0;
 }
 
-// A wave per group.  Lane l has the lists l, l + 64, ..: list = row of the group * slices + slice.
+// The largest of a wave's numbers, through moves between lanes that need no LDS; all lanes get it.
+__device__ __forceinline__ double wave_max_f64(double v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmax(v, __shfl_xor(v, o, 64));
+    return v;
+}
+
+// A wave per group merges the sorted lists (one for each row and slice); lane l has lists l, l + 64, ..
 __global__ __launch_bounds__(64) void beam_merge_kernel(SelectParams p) {
-    extern __shared__ int at[];                    // [lists]: entries taken; then the rows' maxima and log sums
+    extern __shared__ char merge_lds[];
     const int g = blockIdx.x, lane = threadIdx.x, lists = p.W * p.slices;
-    double *base = reinterpret_cast<double *>(at + ((lists + 1) & ~1));      // [W]: score - max - log sum
-    float *row_max = reinterpret_cast<float *>(base + p.W);                   // [W]
+    double *base = reinterpret_cast<double *>(merge_lds);              // [W]: score - log sum
+    float *row_max = reinterpret_cast<float *>(base + p.W);            // [W]; NaN: the row goes by index
+    int *at = reinterpret_cast<int *>(row_max + p.W);                  // [lists]: entries taken
+    uint32_t *held = reinterpret_cast<uint32_t *>(at + lists);         // [lists][n], if they fit
+    const uint32_t *cand = p.cand + (long)g * lists * p.n;
+    if (p.held) {
+        for (int i = lane; i < lists * p.n; i += 64) held[i] = cand[i];
+    }
     for (int i = lane; i < lists; i += 64) at[i] = 0;
     for (int r = lane; r < p.W; r += 64) {
         const long row = (long)g * p.W + r;
         const float score = p.scores[row];
-        const bool ended = p.ended != nullptr && p.ended[row] != 0;
         float m = -INFINITY;
         double s = 0.0;
-        if (score > -INFINITY && !ended) {
+        if (!(score > -INFINITY) || (p.ended != nullptr && p.ended[row] != 0)) {
+            m = __builtin_nanf("");
+            s = 1.0;
+        } else {
             for (int i = 0; i < p.slices; ++i) m = fmaxf(m, p.slice_max[row * p.slices + i]);
             for (int i = 0; i < p.slices; ++i) {
                 const float mi = p.slice_max[row * p.slices + i];
                 s += p.slice_sum[row * p.slices + i] * (mi == m ? 1.0 : exp((double)mi - (double)m));
             }
         }
-        base[r] = (double)score - log(s);
+        // (36 bits of the sum: rows of the same values in another order are equal)
+        base[r] = (double)score - log(__longlong_as_double(__double_as_longlong(s) + (1 << 15) & ~0xFFFFll));
         row_max[r] = m;
     }
     __syncthreads();
-    auto head = [&](int list, double &value, long &index) {            // the list's next candidate
+    constexpr uint32_t NONE = 0xFFFFFFFFu;                             // (beam * vocab + token is below 2^30)
+    auto head = [&](int list, double &value, uint32_t &index) {        // the list's next candidate
         const int r = list / p.slices, slice = list - r * p.slices, i = at[list];
-        const long row = (long)g * p.W + r;
-        const float score = p.scores[row];
-        const bool ended = p.ended != nullptr && p.ended[row] != 0;
+        const float m = row_max[r];
         value = -INFINITY;
-        index = LONG_MAX;
-        if (!(score > -INFINITY) || ended) {       // one list stands for the whole row
+        index = NONE;
+        if (m != m) {                              // one list stands for the whole row
             if (slice != 0 || i >= p.vocab) return;
             int token = i;
-            if (ended && score > -INFINITY) {
+            if (base[r] > -INFINITY) {             // an ended beam: its end, then the others
                 token = i == 0 ? p.eos : i - 1 < p.eos ? i - 1 : i;
-                if (i == 0) value = score;
+                if (i == 0) value = base[r];
             }
-            index = (long)r * p.vocab + token;
+            index = (uint32_t)(r * p.vocab + token);
             return;
         }
-        const uint32_t key = i < p.n ? p.cand[(row * p.slices + slice) * p.n + i] : 0u;
+        const uint32_t key = i >= p.n ? 0u : p.held ? held[list * p.n + i] : cand[(long)list * p.n + i];
         if (key == 0) return;
-        index = (long)r * p.vocab + slice * p.width + (0xFFFFu - (key & 0xFFFFu));
-        const float v = beam_value(key >> 16), m = row_max[r];
-        value = v == -INFINITY ? -INFINITY : base[r] + (v == m ? 0.0 : (double)v - (double)m);
+        index = (uint32_t)(r * p.vocab + slice * p.width + (0xFFFFu - (key & 0xFFFFu)));
+        const float v = beam_value(key >> 16);
+        if (v > -INFINITY) value = base[r] + ((double)v - (double)m);
     };
-    auto better = [](double v, long i, double w, long j) { return v > w || (v == w && i < j); };
     double best = -INFINITY;
-    long index = LONG_MAX;
+    uint32_t index = NONE;
     int list = -1;
     auto mine = [&]() {                            // the best of the lane's lists
         best = -INFINITY;
-        index = LONG_MAX;
-        list = -1;
+        index = NONE;
         for (int i = lane; i < lists; i += 64) {
             double v;
-            long x;
+            uint32_t x;
             head(i, v, x);
-            if (x != LONG_MAX && (list < 0 || better(v, x, best, index))) { best = v; index = x; list = i; }
+            if (x != NONE && (index == NONE || v > best || (v == best && x < index))) { best = v; index = x; list = i; }
         }
     };
     mine();
     for (int k = 0; k < p.n; ++k) {
-        double v = best;
-        long x = index;
+        const double v = wave_max_f64(best);
+        const uint64_t equal = __ballot(best == v && index != NONE);
+        if (equal == 0) break;                     // (not reached: a group has at least n candidates)
+        int lane_of = __ffsll((unsigned long long)equal) - 1;
+        if (equal & (equal - 1)) {                 // equal scores: the lowest index
+            uint32_t x = best == v ? index : NONE;
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            const double w = __shfl_xor(v, o, 64);
-            const long y = __shfl_xor(x, o, 64);
-            if (better(w, y, v, x)) { v = w; x = y; }
+            for (int o = 32; o > 0; o >>= 1) x = min(x, (uint32_t)__shfl_xor((int)x, o, 64));
+            lane_of = __ffsll((unsigned long long)__ballot(index == x)) - 1;
         }
-        if (x == LONG_MAX) x = 0;                  // (not reached: a group has at least n candidates)
-        if (x == index && list >= 0) {
-            at[list] += 1;
-            mine();
-        }
-        if (lane == 0) {
-            const int r = (int)(x / p.vocab), token = (int)(x - (long)r * p.vocab);
+        if (lane == lane_of) {
+            const int r = (int)(index / (uint32_t)p.vocab), token = (int)(index - (uint32_t)r * (uint32_t)p.vocab);
             const long o = (long)g * p.n + k;
             p.out_scores[o] = (float)v;
             p.out_parents[o] = r;
             p.out_tokens[o] = token;
             p.out_ended[o] = token == p.eos || (p.ended != nullptr && p.ended[(long)g * p.W + r] != 0);
+            at[list] += 1;
+            mine();
         }
     }
 }
@@ -234,38 +242,52 @@ struct ReorderParams {
     char *at[REORDER_MAX];
     long stride[REORDER_MAX], bytes[REORDER_MAX];  // from a row to the next; of a row that move
     int unit[REORDER_MAX];                         // > 0: bytes of an entry, of which the first *upto move
+    int piece[REORDER_MAX];                        // bytes that a thread moves at a time: 16 or 4
     int strips[REORDER_MAX];                       // workgroups of the tensors before
     const int32_t *parents, *upto;
-    int W, n, strip;                               // strip: bytes of a row that a workgroup has
+    int W, n, pieces_log2;                         // pieces of a strip
 };
 
-// T: what a thread moves at a time (16 or 4 bytes)
 template <class T>
+__device__ __forceinline__ void reorder_strip(char *base, long stride, T *lds, const int32_t *from, const uint8_t *wanted, int W, int pieces_log2, int pieces) {
+    const int c = threadIdx.x & ((1 << pieces_log2) - 1), r0 = threadIdx.x >> pieces_log2, by = 256 >> pieces_log2;
+    if (c < pieces) {
+#pragma unroll 4
+        for (int r = r0; r < W; r += by)
+            if (wanted[r]) lds[(r << pieces_log2) + c] = *reinterpret_cast<const T *>(base + r * stride + (long)c * sizeof(T));
+    }
+    __syncthreads();
+    if (c < pieces) {
+#pragma unroll 4
+        for (int r = r0; r < W; r += by)
+            if (from[r] != r) *reinterpret_cast<T *>(base + r * stride + (long)c * sizeof(T)) = lds[(from[r] << pieces_log2) + c];
+    }
+}
+
 __global__ __launch_bounds__(256) void beam_reorder_kernel(ReorderParams p) {
-    extern __shared__ char raw[];
+    extern __shared__ u32x4 reorder_lds[];
     __shared__ int32_t from[BEAM_MAX_W];
-    T *lds = reinterpret_cast<T *>(raw);
+    __shared__ uint8_t wanted[BEAM_MAX_W];         // rows that another one takes
     int k = 0;
     for (int i = 1; i < p.n; ++i)
         if ((int)blockIdx.x >= p.strips[i]) k = i;
     const int g = blockIdx.y, t = threadIdx.x, W = p.W;
     long bytes = p.bytes[k];
     if (p.unit[k] > 0) bytes = min(bytes, max((long)p.upto[0], 0L) * p.unit[k]);
-    const long b0 = (long)((int)blockIdx.x - p.strips[k]) * p.strip;
+    const long strip = (long)p.piece[k] << p.pieces_log2, b0 = (long)((int)blockIdx.x - p.strips[k]) * strip;
     if (b0 >= bytes) return;
-    const int per = (int)((min((long)p.strip, bytes - b0) + (long)sizeof(T) - 1) / (long)sizeof(T));      // (a row's bytes are a multiple of T)
-    if (t < W) from[t] = min(max(p.parents[(long)g * W + t], 0), W - 1);
-    __syncthreads();
-    char *base = p.at[k] + (long)g * W * p.stride[k] + b0;
-    for (int i = t; i < W * per; i += 256) {
-        const int r = i / per;
-        lds[i] = *reinterpret_cast<const T *>(base + r * p.stride[k] + (long)(i - r * per) * sizeof(T));
+    const int pieces = (int)(min(strip, bytes - b0) / p.piece[k]);     // (a row's bytes are a multiple of them)
+    const long stride = p.stride[k];
+    if (t < W) {
+        from[t] = min(max(p.parents[(long)g * W + t], 0), W - 1);
+        wanted[t] = 0;
     }
     __syncthreads();
-    for (int i = t; i < W * per; i += 256) {
-        const int r = i / per, f = from[r];
-        if (f != r) *reinterpret_cast<T *>(base + r * p.stride[k] + (long)(i - r * per) * sizeof(T)) = lds[f * per + i - r * per];
-    }
+    if (t < W && from[t] != t) wanted[from[t]] = 1;
+    __syncthreads();
+    char *base = p.at[k] + (long)g * W * stride + b0;
+    if (p.piece[k] == 16) reorder_strip(base, stride, reorder_lds, from, wanted, W, p.pieces_log2, pieces);
+    else reorder_strip(base, stride, reinterpret_cast<uint32_t *>(reorder_lds), from, wanted, W, p.pieces_log2, pieces);
 }
 
 }  // namespace smh
@@ -273,17 +295,18 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(ReorderParams p) {
 using namespace smh;
 
 namespace {
-struct SelectPlan { int slices, width; size_t sums, maxima, cands, bytes; };
-// Slices of 8192 columns where there are rows to fill the GPU with; else of 2048, whose workgroups are done sooner
-SelectPlan select_plan(long rows, int vocab, int n) {
+struct SelectPlan { int slices, width; size_t sums, maxima, cands, bytes, fixed, lists; };
+// Slices of 32768 columns where there are rows to fill the GPU with, of 8192 else (the second launch is short where lists are few)
+SelectPlan select_plan(long rows, int W, int vocab, int n) {
     SelectPlan p;
-    const int wide = (vocab + 8191) / 8192;
-    p.width = rows * wide >= 512 ? 8192 : 2048;
+    p.width = rows * ((vocab + 32767) / 32768) >= 384 && vocab > 8192 && n <= 64 ? 32768 : 8192;      // (64: 32 KB of candidates)
     p.slices = (vocab + p.width - 1) / p.width;
     p.sums = (size_t)rows * p.slices * 8;
     p.maxima = ((size_t)rows * p.slices * 4 + 7) / 8 * 8;
     p.cands = (size_t)rows * p.slices * n * 4;
     p.bytes = p.sums + p.maxima + p.cands;
+    p.fixed = (size_t)W * 12 + (size_t)W * p.slices * 4;               // LDS of the second launch, and of all its lists
+    p.lists = (size_t)W * p.slices * n * 4;
     return p;
 }
 bool select_sizes(int G, int W, int vocab, int n) {
@@ -292,7 +315,7 @@ bool select_sizes(int G, int W, int vocab, int n) {
 }  // namespace
 
 extern "C" size_t smh_beam_select_workspace_bytes(int G, int W, int vocab, int n) {
-    return select_sizes(G, W, vocab, n) ? select_plan((long)G * W, vocab, n).bytes : 0;
+    return select_sizes(G, W, vocab, n) ? select_plan((long)G * W, W, vocab, n).bytes : 0;
 }
 
 extern "C" int smh_beam_select(const void *logits, long ld, const float *scores, const uint8_t *ended, int G, int W, int vocab, int n, int64_t eos, float *out_scores,
@@ -303,13 +326,13 @@ extern "C" int smh_beam_select(const void *logits, long ld, const float *scores,
     SMH_REQUIRE(ld >= vocab, "smh_beam_select: ld=%ld below vocab=%d", ld, vocab);
     SMH_REQUIRE(eos >= 0 && eos < vocab, "smh_beam_select: eos=%ld outside the vocabulary of %d", (long)eos, vocab);
     SMH_REQUIRE(logits && scores && out_scores && out_parents && out_tokens && out_ended, "smh_beam_select: null pointer");
-    const SelectPlan plan = select_plan((long)G * W, vocab, n);
+    const SelectPlan plan = select_plan((long)G * W, W, vocab, n);
     SMH_REQUIRE(W * plan.slices <= BEAM_MAX_LISTS, "smh_beam_select: W=%d beams x %d slices of the vocabulary (at most %d)", W, plan.slices, BEAM_MAX_LISTS);
     SMH_REQUIRE(workspace && ((uintptr_t)workspace & 7) == 0 && workspace_bytes >= plan.bytes, "smh_beam_select: workspace of %zu bytes, %zu needed (8-byte aligned)", workspace_bytes, plan.bytes);
     char *ws = (char *)workspace;
-    SelectParams p{(const half_t *)logits, ld, scores, ended, G * W, W, G, vocab, n, (int)eos, plan.slices, plan.width,
+    const bool held = plan.fixed + plan.lists <= 65536;
+    SelectParams p{(const half_t *)logits, ld, scores, ended, G * W, W, G, vocab, n, (int)eos, plan.slices, plan.width, held,
                    (float *)(ws + plan.sums), (double *)ws, (uint32_t *)(ws + plan.sums + plan.maxima), out_scores, out_parents, out_tokens, out_ended};
-    const dim3 grid(plan.slices, 1, 1);
     const hipStream_t st = (hipStream_t)stream;
     // (rows along y: at most 65535 a launch)
     for (int r = 0; r < G * W; r += 65535) {
@@ -321,12 +344,11 @@ extern "C" int smh_beam_select(const void *logits, long ld, const float *scores,
         part.slice_sum += (long)r * plan.slices;
         part.cand += (long)r * plan.slices * n;
         const int rows = min(65535, G * W - r);
-        if (plan.width == 8192) hipLaunchKernelGGL(beam_slice_kernel<32>, dim3(plan.slices, rows), dim3(256), 0, st, part);
-        else hipLaunchKernelGGL(beam_slice_kernel<8>, dim3(plan.slices, rows), dim3(256), 0, st, part);
+        if (plan.width == 32768) hipLaunchKernelGGL(beam_slice_kernel<16>, dim3(plan.slices, rows), dim3(256), n * 512, st, part);
+        else hipLaunchKernelGGL(beam_slice_kernel<4>, dim3(plan.slices, rows), dim3(256), n * 128, st, part);
         if (int rc = launch_status()) return rc;
     }
-    const size_t lds = (size_t)((W * plan.slices + 1) & ~1) * 4 + (size_t)W * 12;
-    hipLaunchKernelGGL(beam_merge_kernel, dim3(G), dim3(64), lds, st, p);
+    hipLaunchKernelGGL(beam_merge_kernel, dim3(G), dim3(64), plan.fixed + (held ? plan.lists : 0), st, p);
     return launch_status();
 }
 
@@ -341,30 +363,28 @@ extern "C" int smh_beam_reorder(const int32_t *parents, int G, int W, int n, voi
     p.upto = upto;
     p.W = W;
     p.n = n;
-    bool wide = true;
     for (int i = 0; i < n; ++i) {
         SMH_REQUIRE(tensors[i] && bytes[i] >= 0 && strides[i] >= bytes[i] && units[i] >= 0, "smh_beam_reorder: tensor %d: rows of %ld bytes %ld apart, entries of %d", i, bytes[i], strides[i],
                     units[i]);
         SMH_REQUIRE(bytes[i] % 4 == 0 && strides[i] % 4 == 0 && ((uintptr_t)tensors[i] & 3) == 0 && units[i] % 4 == 0, "smh_beam_reorder: tensor %d: rows are multiples of 4 bytes, 4-byte aligned", i);
         SMH_REQUIRE(units[i] == 0 || upto, "smh_beam_reorder: tensor %d goes by *upto, which is null", i);
         for (int j = 0; j < i; ++j) SMH_REQUIRE(tensors[i] != tensors[j], "smh_beam_reorder: tensors %d and %d are the same", j, i);
-        wide = wide && bytes[i] % 16 == 0 && strides[i] % 16 == 0 && ((uintptr_t)tensors[i] & 15) == 0 && (units[i] == 0 || bytes[i] >= 0);
     }
-    for (int i = 0; i < n; ++i) wide = wide && units[i] == 0;
-    p.strip = wide ? 512 : 256;
+    // a strip of a group is at most 64 KB of LDS: 256 pieces of 16 bytes up to 16 beams, 64 of 64
+    p.pieces_log2 = W <= 16 ? 8 : W <= 32 ? 7 : 6;
     long strips = 0;
     for (int i = 0; i < n; ++i) {
         p.at[i] = (char *)tensors[i];
         p.stride[i] = strides[i];
         p.bytes[i] = bytes[i];
         p.unit[i] = units[i];
+        p.piece[i] = units[i] == 0 && bytes[i] % 16 == 0 && strides[i] % 16 == 0 && ((uintptr_t)tensors[i] & 15) == 0 ? 16 : 4;
         p.strips[i] = (int)strips;
-        strips += (bytes[i] + p.strip - 1) / p.strip;
+        const long strip = (long)p.piece[i] << p.pieces_log2;
+        strips += (bytes[i] + strip - 1) / strip;
         SMH_REQUIRE(strips < (1L << 31), "smh_beam_reorder: rows too long");
     }
     if (strips == 0) return 0;
-    const size_t lds = (size_t)W * p.strip;
-    if (wide) hipLaunchKernelGGL(beam_reorder_kernel<u32x4>, dim3((unsigned)strips, G), dim3(256), lds, (hipStream_t)stream, p);
-    else hipLaunchKernelGGL(beam_reorder_kernel<uint32_t>, dim3((unsigned)strips, G), dim3(256), lds, (hipStream_t)stream, p);
+    hipLaunchKernelGGL(beam_reorder_kernel, dim3((unsigned)strips, G), dim3(256), ((size_t)W * 16) << p.pieces_log2, (hipStream_t)stream, p);
     return launch_status();
 }

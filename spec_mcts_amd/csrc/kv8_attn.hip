@@ -426,9 +426,9 @@ __global__ __launch_bounds__(256) void kv8_attn_many_kernel(Kv8AttnParams p) {
     }
 }
 
-// The parts of each query: half a wave a query, four dims a lane.
+// The parts of each query: a wave a query.  Lanes have the parts' (m, l) first, 64 at a time, then half a wave a part's sums, four dims a lane.
 __global__ __launch_bounds__(256) void kv8_attn_merge_kernel(Kv8AttnParams p) {
-    const long rows = (long)p.T * p.H, r = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const long rows = (long)p.T * p.H, r = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (r >= rows) return;
     if (p.cu != nullptr) {                         // rows of no sequence (behind the last one, past max_new) have no parts
         const int tok = (int)(r / p.H);
@@ -441,18 +441,49 @@ __global__ __launch_bounds__(256) void kv8_attn_merge_kernel(Kv8AttnParams p) {
         const Kv8Seq s = kv8_seq(p.lens, p.cu, lo, p.T, p.max_new);
         if (tok < s.t0 || tok >= s.t0 + s.n) return;
     }
-    const int d = (threadIdx.x & 31) * 4;
-    float top = -INFINITY, l = 0.0f;
-    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, p.part_ml[s * rows + r].x);
-    const float zero = top == -INFINITY ? 0.0f : top;
-    f4 a = {0, 0, 0, 0};
-    for (int s = 0; s < p.splits; ++s) {
-        const float2 ml = p.part_ml[s * rows + r];
-        if (ml.x == -INFINITY) continue;           // (no sums were left)
-        const float by = __builtin_amdgcn_exp2f(ml.x - zero);
-        l += ml.y * by;
-        a += *reinterpret_cast<const f4 *>(p.part_o + (s * rows + r) * KV8_DIM + d) * by;
+    const int lane = threadIdx.x & 63, half = lane >> 5, d = (lane & 31) * 4;
+    float m[4], l = 0.0f, w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        m[k] = -INFINITY;
+        w[k] = 0.0f;
+        const int s = k * 64 + lane;
+        if (s < p.splits) {
+            const float2 ml = p.part_ml[s * rows + r];
+            m[k] = ml.x;
+            w[k] = ml.y;
+        }
     }
+    const float top = wave_max(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]))), zero = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float by = __builtin_amdgcn_exp2f(m[k] - zero);          // (0 for a part that saw nothing: no sums were left)
+        l += m[k] == -INFINITY ? 0.0f : w[k] * by;
+        w[k] = by;
+    }
+    l = wave_sum(l);
+    f4 a = {0, 0, 0, 0};
+    const float *o = p.part_o + r * KV8_DIM + d;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int n = min(p.splits - k * 64, 64);
+        for (int s0 = 0; s0 < n; s0 += 16) {
+            f4 x[8];
+            float by[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int s = s0 + i * 2 + half;
+                by[i] = __shfl(w[k], s & 63, 64);
+                x[i] = f4{0, 0, 0, 0};
+                if (s < n && by[i] != 0.0f) x[i] = *reinterpret_cast<const f4 *>(o + (k * 64 + s) * rows * KV8_DIM);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a += x[i] * (s0 + i * 2 + half < n ? by[i] : 0.0f);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) a[e] += __shfl_xor(a[e], 32, 64);
+    if (half != 0) return;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     h4 y;
 #pragma unroll
@@ -539,7 +570,7 @@ extern "C" int smh_kv8_attn(const void *q, void *out, int T, int B, int H, int H
     if (int rc = launch_status()) return rc;
     if (plan.splits == 1) return 0;
     const long rows = (long)T * H;
-    SMH_REQUIRE((rows + 7) / 8 < (1L << 31), "smh_kv8_attn: T=%d", T);
-    hipLaunchKernelGGL(kv8_attn_merge_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, p);
+    SMH_REQUIRE((rows + 3) / 4 < (1L << 31), "smh_kv8_attn: T=%d", T);
+    hipLaunchKernelGGL(kv8_attn_merge_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p);
     return launch_status();
 }

@@ -43,14 +43,22 @@ __device__ __forceinline__ uint32_t abs_max8(uint32_t m, h8 x) {      // of the 
     for (int i = 0; i < 4; ++i) m = max(m, max(w[i] & 0x7FFFu, (w[i] >> 16) & 0x7FFFu));
     return m;
 }
-// The largest of 256 threads.  `red`: 4 words of LDS, free when it is called.
-__device__ __forceinline__ float block_amax(uint32_t m, uint32_t *red) {
+// The largest of 256 threads, of two numbers each.  `red`: 8 words of LDS.
+__device__ __forceinline__ void block_amax(uint32_t a, uint32_t b, uint32_t *red, float &fa, float &fb) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+    for (int o = 32; o > 0; o >>= 1) {
+        a = max(a, (uint32_t)__shfl_xor((int)a, o, 64));
+        b = max(b, (uint32_t)__shfl_xor((int)b, o, 64));
+    }
+    if ((threadIdx.x & 63) == 0) {
+        red[threadIdx.x >> 6] = a;
+        red[4 + (threadIdx.x >> 6)] = b;
+    }
     __syncthreads();
-    m = max(max(red[0], red[1]), max(red[2], red[3]));
-    return (float)__builtin_bit_cast(half_t, (uint16_t)m);
+    a = max(max(red[0], red[1]), max(red[2], red[3]));
+    b = max(max(red[4], red[5]), max(red[6], red[7]));
+    fa = (float)__builtin_bit_cast(half_t, (uint16_t)a);
+    fb = (float)__builtin_bit_cast(half_t, (uint16_t)b);
 }
 // (an infinity or a NaN among the values: the scale is NaN, and the block's values with it; the codes stay codes)
 __device__ __forceinline__ uint32_t kv8_code(half_t x, float inverse) {
@@ -61,36 +69,40 @@ __device__ __forceinline__ float kv8_inverse(float amax) { return amax > 0.0f ? 
 
 constexpr int V_PITCH = 17;                        // words of LDS a line of V's codes takes: 16 and one, against bank conflicts
 
-// One block of K and V of a head becomes codes.  row_k, row_v: (row of the block) -> eight dims of it, for the thread's dims.  256 threads: thread t has rows
-// 4 (t / 16) .. + 3 and dims 8 (t % 16) .. + 7.
-template <class RK, class RV>
-__device__ __forceinline__ void kv8_quantize_block(const Kv8Cache &c, long tile, RK row_k, RV row_v, uint32_t *lds, uint32_t *red) {
-    const int t = threadIdx.x, quad = t >> 4, dc = t & 15;
-    h8 x[4];
-    uint32_t m = 0;
+// Eight dims of four rows of an open V block: four places of eight lines
+__device__ __forceinline__ void open_v_rows(const half_t *open_v, int quad, int dc, h8 (&x)[4]) {
+    const half_t *at = open_v + dc * 8 * KV8_ROWS + kv8_place(quad * 4);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { x[i] = row_k(quad * 4 + i); m = abs_max8(m, x[i]); }
-    const float ak = block_amax(m, red);
-    const float ik = kv8_inverse(ak);
+    for (int e = 0; e < 8; ++e) {
+        const h4 y = *reinterpret_cast<const h4 *>(at + e * KV8_ROWS);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i][e] = y[i];
+    }
+}
+
+// One block of K and V of a head becomes codes.  256 threads: thread t has rows 4 (t / 16) .. + 3 and dims 8 (t % 16) .. + 7, k[i] and v[i] of row i of them.
+__device__ __forceinline__ void kv8_quantize_block(const Kv8Cache &c, long tile, const h8 (&k_rows)[4], const h8 (&v_rows)[4], uint32_t *lds, uint32_t *red) {
+    const int t = threadIdx.x, quad = t >> 4, dc = t & 15;
+    uint32_t mk = 0, mv = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { mk = abs_max8(mk, k_rows[i]); mv = abs_max8(mv, v_rows[i]); }
+    float ak, av;
+    block_amax(mk, mv, red, ak, av);
+    const float ik = kv8_inverse(ak), iv = kv8_inverse(av);
     uint8_t *k = c.k + tile * KV8_TILE;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         u32x2 w = {0, 0};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[e >> 2] |= kv8_code(x[i][e], ik) << (8 * (e & 3));
+        for (int e = 0; e < 8; ++e) w[e >> 2] |= kv8_code(k_rows[i][e], ik) << (8 * (e & 3));
         *reinterpret_cast<u32x2 *>(k + (quad * 4 + i) * KV8_DIM + dc * 8) = w;
     }
-    m = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { x[i] = row_v(quad * 4 + i); m = abs_max8(m, x[i]); }
-    const float av = block_amax(m, red + 4);
-    const float iv = kv8_inverse(av);
     const int word = kv8_place(quad * 4) >> 2;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         uint32_t w = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w |= kv8_code(x[i][e], iv) << (8 * i);
+        for (int i = 0; i < 4; ++i) w |= kv8_code(v_rows[i][e], iv) << (8 * i);
         lds[(dc * 8 + e) * V_PITCH + word] = w;
     }
     __syncthreads();
@@ -124,21 +136,29 @@ __global__ __launch_bounds__(256) void kv8_append_one_kernel(AppendParams p) {
     const int kvh = blockIdx.x, b = blockIdx.y;
     const Kv8Seq s = kv8_seq(p.lens, p.cu, b, p.T, 1);
     if (s.n == 0) return;
-    const int t = threadIdx.x, c = t & 15, n_rep = p.H / p.Hkv;
+    const int t = threadIdx.x, c = t & 15, quad = t >> 4, n_rep = p.H / p.Hkv;
     const int at = min(s.old, p.table_rows - 1), row = s.old & 63;
     const half_t *cs = p.cos_tab + (long)at * 64, *sn = p.sin_tab + (long)at * 64;
-    const bool whole = row == 63;
     const long head = (long)b * p.Hkv + kvh;
-    for (int r = t >> 4; r < n_rep + 2; r += 16) {
+    half_t *open_k = p.c.open_k + head * KV8_TILE, *open_v = p.c.open_v + head * KV8_TILE;
+    // The 64th row of its block: the other 63 are asked for with it
+    const long page = row == 63 ? kv8_page_to_write(p.c, b, s.old >> 6) : -1;
+    h8 xk[4], xv[4];
+    if (page >= 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) xk[i] = *reinterpret_cast<const h8 *>(open_k + (quad * 4 + i) * KV8_DIM + c * 8);
+        open_v_rows(open_v, quad, c, xv);
+    }
+    for (int r = quad; r < n_rep + 2; r += 16) {
         if (r == 0) {
             const h8 x = rope8(*reinterpret_cast<const h8 *>(p.k + s.t0 * p.k_stride + kvh * KV8_DIM + c * 8), cs, sn, c);
-            if (whole) fresh[0][c] = x;
-            else if ((s.old >> 6) <= p.c.cols) *reinterpret_cast<h8 *>(p.c.open_k + head * KV8_TILE + row * KV8_DIM + c * 8) = x;
+            if (row == 63) fresh[0][c] = x;
+            else if ((s.old >> 6) <= p.c.cols) *reinterpret_cast<h8 *>(open_k + row * KV8_DIM + c * 8) = x;
         } else if (r == 1) {
             const h8 x = *reinterpret_cast<const h8 *>(p.v + s.t0 * p.v_stride + kvh * KV8_DIM + c * 8);
-            if (whole) fresh[1][c] = x;
+            if (row == 63) fresh[1][c] = x;
             else if ((s.old >> 6) <= p.c.cols) {
-                half_t *at_v = p.c.open_v + head * KV8_TILE + kv8_place(row);
+                half_t *at_v = open_v + kv8_place(row);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) at_v[(c * 8 + e) * KV8_ROWS] = x[e];
             }
@@ -148,28 +168,13 @@ __global__ __launch_bounds__(256) void kv8_append_one_kernel(AppendParams p) {
             *reinterpret_cast<h8 *>(p.q_out + ((long)s.t0 * p.H + h) * KV8_DIM + c * 8) = rope8(x, cs, sn, c);
         }
     }
-    if (!whole) return;
-    const long page = kv8_page_to_write(p.c, b, s.old >> 6);
     if (page < 0) return;
     __syncthreads();
-    const half_t *open_k = p.c.open_k + head * KV8_TILE, *open_v = p.c.open_v + head * KV8_TILE;
-    kv8_quantize_block(
-        p.c, page * p.Hkv + kvh,
-        [&](int r) {
-            u32x4 x = *reinterpret_cast<const u32x4 *>(open_k + r * KV8_DIM + c * 8);
-            asm("" : "+v"(x));                     // (a choice between two values, not a load from a chosen memory)
-            if (r == 63) x = __builtin_bit_cast(u32x4, fresh[0][c]);
-            return __builtin_bit_cast(h8, x);
-        },
-        [&](int r) {
-            if (r == 63) return fresh[1][c];
-            h8 x;
-            const int place = kv8_place(r);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = open_v[(c * 8 + e) * KV8_ROWS + place];
-            return x;
-        },
-        lds, red);
+    if (quad == 15) {
+        xk[3] = fresh[0][c];
+        xv[3] = fresh[1][c];
+    }
+    kv8_quantize_block(p.c, page * p.Hkv + kvh, xk, xv, lds, red);
 }
 
 // Any number of new rows: a workgroup has one block and kv head, or 64 new rows of one query head.
@@ -223,22 +228,19 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendParams p) {
     const long page = kv8_page_to_write(p.c, b, j);
     if (page >= 0) {
         const int before = s.old - j * KV8_ROWS;          // rows of the block that were there
-        kv8_quantize_block(
-            p.c, page * p.Hkv + kvh,
-            [&](int r) {
-                const long i = r - before;
-                return i < 0 ? *reinterpret_cast<const h8 *>(open_k + r * KV8_DIM + c * 8) : rotated(k + i * p.k_stride, (int)i);
-            },
-            [&](int r) {
-                const long i = r - before;
-                if (i >= 0) return *reinterpret_cast<const h8 *>(v + i * p.v_stride + c * 8);
-                h8 x;
-                const int place = kv8_place(r);
+        h8 xk[4], xv[4];
+        if (quad * 4 < before) open_v_rows(open_v, quad, c, xv);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = open_v[(c * 8 + e) * KV8_ROWS + place];
-                return x;
-            },
-            lds, red);
+        for (int e = 0; e < 4; ++e) {
+            const int r = quad * 4 + e;
+            const long i = r - before;
+            if (i < 0) xk[e] = *reinterpret_cast<const h8 *>(open_k + r * KV8_DIM + c * 8);
+            else {
+                xk[e] = rotated(k + i * p.k_stride, (int)i);
+                xv[e] = *reinterpret_cast<const h8 *>(v + i * p.v_stride + c * 8);
+            }
+        }
+        kv8_quantize_block(p.c, page * p.Hkv + kvh, xk, xv, lds, red);
     }
     if (both && blockIdx.x == 0) {
         __syncthreads();

@@ -177,7 +177,7 @@ def test_workspaces():
 
 @pytest.mark.parametrize("bad,why", [(dict(W=65), b"beams"), (dict(W=0), b"beams"), (dict(n=0), b"n="), (dict(n=129), b"n="), (dict(n=100, vocab=99, ld=99), b"n="), (dict(G=0), b"G="),
                                      (dict(ld=40), b"ld="), (dict(eos=-1), b"eos"), (dict(eos=50), b"eos"), (dict(logits=None), b"null"), (dict(ws=None), b"workspace"),
-                                     (dict(ws_bytes=8), b"workspace"), (dict(ws=(1 << 20) + 4), b"workspace"), (dict(vocab=1 << 24, ld=1 << 24), b"slices")], ids=str)
+                                     (dict(ws_bytes=8), b"workspace"), (dict(ws=(1 << 20) + 4), b"workspace"), (dict(W=64, vocab=1 << 24, ld=1 << 24), b"slices")], ids=str)
 def test_c_select_refuses(bad, why):
     a = dict(logits=1 << 21, ld=50, scores=1 << 12, ended=None, G=2, W=3, vocab=50, n=4, eos=2, o0=1 << 13, o1=1 << 14, o2=1 << 15, o3=1 << 16, ws=1 << 20, ws_bytes=1 << 40, stream=None)
     a.update(bad)
