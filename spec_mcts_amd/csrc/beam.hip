@@ -1,14 +1,16 @@
 // Beam search: the best continuations of each group of beams, and the states that follow them.
 //
 // Selection.  Candidate (beam r, token t) of a group has the score  scores[r] + x[r][t] - log sum_t' exp(x[r][t']);  the n best leave in descending order,
-// equal ones by (beam, token).  A first launch goes over each row once, a workgroup per slice of it: the slice's values stay in registers while its maximum, its sum of
-// exponentials and its n largest values are found.  A second one has a wave per group: it adds the slices' sums up and merges their sorted lists.
+// equal ones by (beam, token).  A first launch goes over each row once, a workgroup per slice of it: the slice's values stay in registers while its n largest, its maximum and its
+// sum of exponentials are found.  A second one has a workgroup per group: it adds the slices' sums up and picks the n best of all lists (one step a bit of the score,
+// ended when just n are left above).
 //   Order: within a row the fp16 values order exactly; between rows the scores are compared in 64 bits, with sums in 64 bits of fp32 terms, so that
 //   candidates keep their order unless they are closer than the terms' roundings (2^-24 each) leave the sums.
-// Bound: HBM, 2 bytes a logit; the smallest calls by the two launches.
+// Bound: 2 bytes a logit from HBM; short of that by the exponentials and their 64-bit sums (512 rows of 32016: 18 us for the first launch, of which HBM needs 6.6) and, for few rows, by
+// two launches (4 rows: 6.6 and 5.0 us).
 //
 // Reordering.  Row i of a group takes the contents of row parents[i], in place: a workgroup owns a strip of all rows of a group, has it in LDS and then writes.
-// Bound: HBM, each row that moves read and written once.
+// Bound: HBM, each row that another one takes read and each row that changes written once (64 rows of four layers' open blocks, 2 MB each, 17.5 us; 73 with four bytes a thread at a time).
 #include "smh_common.hpp"
 
 namespace smh {
@@ -20,7 +22,7 @@ struct SelectParams {
     long ld;
     const float *scores;
     const uint8_t *ended;                          // may be null
-    int rows, W, G, vocab, n, eos, slices, width, held;      // width: columns of a slice; held: the second launch has all lists in LDS
+    int rows, W, G, vocab, n, eos, slices, width;  // width: columns of a slice
     float *slice_max;                              // [rows][slices]
     double *slice_sum;                             // [rows][slices], of exp(x - slice_max)
     uint32_t *cand;                                // [rows][slices][n]: keys (below), descending; 0: none
@@ -67,16 +69,18 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(SelectParams p) {
                 if (col + e < cols) v[i][e] = x[col + e];
         }
     }
+    auto chunk_key = [](h8 v, uint32_t chunk) {
+        const h4 a = __builtin_elementwise_max(__builtin_shufflevector(v, v, 0, 1, 2, 3), __builtin_shufflevector(v, v, 4, 5, 6, 7));
+        const h2 b = __builtin_elementwise_max(__builtin_shufflevector(a, a, 0, 1), __builtin_shufflevector(a, a, 2, 3));
+        const half_t m = __builtin_elementwise_max(b[0], b[1]) + (half_t)0.0f;      // (+ 0: one zero)
+        return beam_order(m) << 16 | (0xFFFFu - chunk);
+    };
     // the thread's key: order of its largest value, then the chunks' order (they are in the columns' order), 0 without columns
     uint32_t mine = 0;
 #pragma unroll
     for (int i = 0; i < CHUNKS; ++i) {
         v[i] = __builtin_elementwise_max(v[i], least);                 // (NaN: -infinity)
-        const h4 a = __builtin_elementwise_max(__builtin_shufflevector(v[i], v[i], 0, 1, 2, 3), __builtin_shufflevector(v[i], v[i], 4, 5, 6, 7));
-        const h2 b = __builtin_elementwise_max(__builtin_shufflevector(a, a, 0, 1), __builtin_shufflevector(a, a, 2, 3));
-        const half_t m = __builtin_elementwise_max(b[0], b[1]) + (half_t)0.0f;      // (+ 0: one zero)
-        const uint32_t key = beam_order(m) << 16 | (0xFFFFu - (uint32_t)(i * 256 + t));
-        if ((i * 256 + t) * 8 < cols) mine = max(mine, key);
+        if ((i * 256 + t) * 8 < cols) mine = max(mine, chunk_key(v[i], i * 256 + t));
     }
     top[t] = mine;
     if (t == 0) n_found = 0;
@@ -86,18 +90,19 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(SelectParams p) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) mx[i] = top[i * 64 + lane];
     uint32_t bar = 0;
-#pragma unroll
     for (int bit = 31; bit >= 0; --bit) {
         const uint32_t at = bar | 1u << bit;
         int c = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) c += __popcll(__ballot(mx[i] >= at));
         if (c >= n) bar = at;
+        if (c == n) break;                         // (just n are not below it already)
     }
     if (mine >= bar && mine != 0) {
 #pragma unroll
         for (int i = 0; i < CHUNKS; ++i) {
             const uint32_t chunk = i * 256 + t;
+            if (chunk_key(v[i], chunk) < bar) continue;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const uint32_t order = beam_order(v[i][e] + (half_t)0.0f);
@@ -112,10 +117,16 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(SelectParams p) {
     // exp(x - m): the difference is exact or rounded once, its product with log2(e) is off by 2^-24 of itself, so terms near the largest have 2^-23
     double total = 0.0;
     if (m > -INFINITY) {
+        auto add = [&](float x) { total += (double)__builtin_amdgcn_exp2f((x - m) * 1.44269504f); };
+        if (m < 65536.0f) {
 #pragma unroll
-        for (int i = 0; i < CHUNKS; ++i)
+            for (int i = 0; i < CHUNKS; ++i)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) total += (double)__builtin_amdgcn_exp2f((fminf((float)v[i][e], 65536.0f) - m) * 1.44269504f);
+                for (int e = 0; e < 8; ++e) add((float)v[i][e]);
+        } else {                                   // some are infinite
+            for (int i = 0; i < CHUNKS; ++i)
+                for (int e = 0; e < 8; ++e) add(fminf((float)v[i][e], 65536.0f));
+        }
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
@@ -136,100 +147,175 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(SelectParams p) {
     for (int i = have + t; i < n; i += 256) cand[i] = 0;
 }
 
-// The largest of a wave's numbers, through moves between lanes that need no LDS; all lanes get it.
+// What the second launch knows of a row
+struct BeamRow { double base; float max; };        // score - log sum (of an ended beam the score); the largest logit, NaN: the row's candidates go by index
+__device__ __forceinline__ BeamRow beam_row(const SelectParams &p, long row) {
+    const float score = p.scores[row];
+    if (!(score > -INFINITY) || (p.ended != nullptr && p.ended[row] != 0)) return BeamRow{(double)score, __builtin_nanf("")};
+    float m = -INFINITY;
+    double s = 0.0;
+    for (int i = 0; i < p.slices; ++i) m = fmaxf(m, p.slice_max[row * p.slices + i]);
+    for (int i = 0; i < p.slices; ++i) {
+        const float mi = p.slice_max[row * p.slices + i];
+        s += p.slice_sum[row * p.slices + i] * (mi == m ? 1.0 : exp((double)mi - (double)m));
+    }
+    // (36 bits of the sum: rows of the same values in another order are equal)
+    return BeamRow{(double)score - log(__longlong_as_double((__double_as_longlong(s) + (1 << 15)) & ~0xFFFFll)), m};
+}
+constexpr uint32_t BEAM_NONE = 0xFFFFFFFFu;        // (beam * vocab + token is below 2^30)
+// Candidate i of list (row r, slice) with its key: score and index; BEAM_NONE: there is none
+__device__ __forceinline__ void beam_candidate(const SelectParams &p, const BeamRow &row, int r, int slice, int i, uint32_t key, double &value, uint32_t &index) {
+    value = -INFINITY;
+    index = BEAM_NONE;
+    if (row.max != row.max) {                      // one list stands for the whole row
+        if (slice != 0 || i >= p.vocab) return;
+        int token = i;
+        if (row.base > -INFINITY) {                // an ended beam: its end, then the others
+            token = i == 0 ? p.eos : i - 1 < p.eos ? i - 1 : i;
+            if (i == 0) value = row.base;
+        }
+        index = (uint32_t)(r * p.vocab + token);
+        return;
+    }
+    if (key == 0) return;
+    index = (uint32_t)(r * p.vocab + slice * p.width + (0xFFFFu - (key & 0xFFFFu)));
+    const float v = beam_value(key >> 16);
+    if (v > -INFINITY) value = row.base + ((double)v - (double)row.max);
+}
+__device__ __forceinline__ void beam_out(const SelectParams &p, int g, int k, double value, uint32_t index) {
+    const int r = (int)(index / (uint32_t)p.vocab), token = (int)(index - (uint32_t)r * (uint32_t)p.vocab);
+    const long o = (long)g * p.n + k;
+    p.out_scores[o] = (float)value;
+    p.out_parents[o] = r;
+    p.out_tokens[o] = token;
+    p.out_ended[o] = token == p.eos || (p.ended != nullptr && p.ended[(long)g * p.W + r] != 0);
+}
+// 64 bits that order as the numbers do
+__device__ __forceinline__ uint64_t ordered64(double v) {
+    const uint64_t b = (uint64_t)__double_as_longlong(v == 0.0 ? 0.0 : v);
+    return b >> 63 ? ~b : b | 1ull << 63;
+}
+__device__ __forceinline__ double unordered64(uint64_t o) { return __longlong_as_double((long long)(o >> 63 ? o & ~(1ull << 63) : ~o)); }
+
+// A workgroup per group has all candidates, K of them a thread, and finds the n-th largest score bit by bit; among equal ones at the border the lowest indices stay.
+template <int K, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void beam_pick_kernel(SelectParams p) {
+    __shared__ BeamRow rows[BEAM_MAX_W];
+    __shared__ uint64_t best[BEAM_MAX_N];
+    __shared__ uint32_t best_index[BEAM_MAX_N];
+    __shared__ int counts[2][WAVES], have;
+    const int g = blockIdx.x, t = threadIdx.x, wave = t >> 6, all = p.W * p.slices * p.n, n = p.n;
+    const uint32_t *cand = p.cand + (long)g * all;
+    uint32_t key[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) key[k] = (k * WAVES * 64 + t) < all ? cand[k * WAVES * 64 + t] : 0u;
+    if (t < p.W) rows[t] = beam_row(p, (long)g * p.W + t);
+    if (t == 0) have = 0;
+    __syncthreads();
+    uint64_t score[K];                             // 0: no candidate (a number's is larger)
+    uint32_t index[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int c = k * WAVES * 64 + t, list = c / n, r = list / p.slices;
+        double v = -INFINITY;
+        index[k] = BEAM_NONE;
+        if (c < all) beam_candidate(p, rows[r], r, list - r * p.slices, c - list * n, key[k], v, index[k]);
+        score[k] = index[k] == BEAM_NONE ? 0 : ordered64(v);
+    }
+    int turn = 0;
+    auto count = [&](auto test) {                  // of all threads' candidates
+        int c = 0;
+#pragma unroll
+        for (int k = 0; k < K; ++k) c += __popcll(__ballot(test(k)));
+        if (WAVES > 1) {                           // (two sets: who writes one has passed the barrier behind the last reads of it)
+            if ((t & 63) == 0) counts[turn][wave] = c;
+            __syncthreads();
+            c = 0;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) c += counts[turn][w];
+            turn ^= 1;
+        }
+        return c;
+    };
+    uint64_t bar = 0;
+    bool exact = false;                            // just n scores are not below the bar
+    for (int bit = 63; bit >= 0 && !exact; --bit) {
+        const uint64_t at = bar | 1ull << bit;
+        const int c = count([&](int k) { return score[k] >= at; });
+        if (c >= n) bar = at;
+        exact = c == n;
+    }
+    uint32_t last = BEAM_NONE - 1;                 // the last index that stays of the scores that are the bar
+    if (!exact) {
+        const int left = n - count([&](int k) { return score[k] > bar; });
+        last = 0;                                  // the left-th smallest index: the largest with fewer than `left` below it
+        for (int bit = 29; bit >= 0; --bit) {
+            const uint32_t at = last | 1u << bit;
+            if (count([&](int k) { return score[k] == bar && index[k] < at; }) < left) last = at;
+        }
+    }
+    // those n, in any order, and the place of each
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+        if (score[k] != 0 && (exact ? score[k] >= bar : score[k] > bar || (score[k] == bar && index[k] <= last))) {
+            const int at = atomicAdd(&have, 1);
+            if (at < n) { best[at] = score[k]; best_index[at] = index[k]; }
+        }
+    __syncthreads();
+    const int found = min(have, n);                // (n: a group has at least that many)
+    for (int i = t; i < found; i += 64 * WAVES) {
+        const uint64_t s = best[i];
+        const uint32_t x = best_index[i];
+        int above = 0;
+        for (int j = 0; j < found; ++j) above += best[j] > s || (best[j] == s && best_index[j] < x);
+        beam_out(p, g, above, unordered64(s), x);
+    }
+}
+
+// The largest of a wave's numbers
 __device__ __forceinline__ double wave_max_f64(double v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v = fmax(v, __shfl_xor(v, o, 64));
     return v;
 }
 
-// A wave per group merges the sorted lists (one for each row and slice); lane l has lists l, l + 64, ..
+// More candidates than that: a wave per group merges the sorted lists (one for each row and slice); lane l has lists l, l + 64, ..
 __global__ __launch_bounds__(64) void beam_merge_kernel(SelectParams p) {
-    extern __shared__ char merge_lds[];
+    extern __shared__ int at[];                    // [lists]: entries taken
+    __shared__ BeamRow rows[BEAM_MAX_W];
     const int g = blockIdx.x, lane = threadIdx.x, lists = p.W * p.slices;
-    double *base = reinterpret_cast<double *>(merge_lds);              // [W]: score - log sum
-    float *row_max = reinterpret_cast<float *>(base + p.W);            // [W]; NaN: the row goes by index
-    int *at = reinterpret_cast<int *>(row_max + p.W);                  // [lists]: entries taken
-    uint32_t *held = reinterpret_cast<uint32_t *>(at + lists);         // [lists][n], if they fit
     const uint32_t *cand = p.cand + (long)g * lists * p.n;
-    if (p.held) {
-        for (int i = lane; i < lists * p.n; i += 64) held[i] = cand[i];
-    }
     for (int i = lane; i < lists; i += 64) at[i] = 0;
-    for (int r = lane; r < p.W; r += 64) {
-        const long row = (long)g * p.W + r;
-        const float score = p.scores[row];
-        float m = -INFINITY;
-        double s = 0.0;
-        if (!(score > -INFINITY) || (p.ended != nullptr && p.ended[row] != 0)) {
-            m = __builtin_nanf("");
-            s = 1.0;
-        } else {
-            for (int i = 0; i < p.slices; ++i) m = fmaxf(m, p.slice_max[row * p.slices + i]);
-            for (int i = 0; i < p.slices; ++i) {
-                const float mi = p.slice_max[row * p.slices + i];
-                s += p.slice_sum[row * p.slices + i] * (mi == m ? 1.0 : exp((double)mi - (double)m));
-            }
-        }
-        // (36 bits of the sum: rows of the same values in another order are equal)
-        base[r] = (double)score - log(__longlong_as_double(__double_as_longlong(s) + (1 << 15) & ~0xFFFFll));
-        row_max[r] = m;
-    }
+    if (lane < p.W) rows[lane] = beam_row(p, (long)g * p.W + lane);
     __syncthreads();
-    constexpr uint32_t NONE = 0xFFFFFFFFu;                             // (beam * vocab + token is below 2^30)
-    auto head = [&](int list, double &value, uint32_t &index) {        // the list's next candidate
-        const int r = list / p.slices, slice = list - r * p.slices, i = at[list];
-        const float m = row_max[r];
-        value = -INFINITY;
-        index = NONE;
-        if (m != m) {                              // one list stands for the whole row
-            if (slice != 0 || i >= p.vocab) return;
-            int token = i;
-            if (base[r] > -INFINITY) {             // an ended beam: its end, then the others
-                token = i == 0 ? p.eos : i - 1 < p.eos ? i - 1 : i;
-                if (i == 0) value = base[r];
-            }
-            index = (uint32_t)(r * p.vocab + token);
-            return;
-        }
-        const uint32_t key = i >= p.n ? 0u : p.held ? held[list * p.n + i] : cand[(long)list * p.n + i];
-        if (key == 0) return;
-        index = (uint32_t)(r * p.vocab + slice * p.width + (0xFFFFu - (key & 0xFFFFu)));
-        const float v = beam_value(key >> 16);
-        if (v > -INFINITY) value = base[r] + ((double)v - (double)m);
-    };
     double best = -INFINITY;
-    uint32_t index = NONE;
+    uint32_t index = BEAM_NONE;
     int list = -1;
-    auto mine = [&]() {                            // the best of the lane's lists
+    auto mine = [&]() {                            // the best of the lane's lists' next candidates
         best = -INFINITY;
-        index = NONE;
+        index = BEAM_NONE;
         for (int i = lane; i < lists; i += 64) {
+            const int r = i / p.slices, e = at[i];
             double v;
             uint32_t x;
-            head(i, v, x);
-            if (x != NONE && (index == NONE || v > best || (v == best && x < index))) { best = v; index = x; list = i; }
+            beam_candidate(p, rows[r], r, i - r * p.slices, e, e < p.n ? cand[(long)i * p.n + e] : 0u, v, x);
+            if (x != BEAM_NONE && (index == BEAM_NONE || v > best || (v == best && x < index))) { best = v; index = x; list = i; }
         }
     };
     mine();
     for (int k = 0; k < p.n; ++k) {
         const double v = wave_max_f64(best);
-        const uint64_t equal = __ballot(best == v && index != NONE);
+        const uint64_t equal = __ballot(best == v && index != BEAM_NONE);
         if (equal == 0) break;                     // (not reached: a group has at least n candidates)
         int lane_of = __ffsll((unsigned long long)equal) - 1;
         if (equal & (equal - 1)) {                 // equal scores: the lowest index
-            uint32_t x = best == v ? index : NONE;
+            uint32_t x = best == v ? index : BEAM_NONE;
 #pragma unroll
             for (int o = 32; o > 0; o >>= 1) x = min(x, (uint32_t)__shfl_xor((int)x, o, 64));
             lane_of = __ffsll((unsigned long long)__ballot(index == x)) - 1;
         }
         if (lane == lane_of) {
-            const int r = (int)(index / (uint32_t)p.vocab), token = (int)(index - (uint32_t)r * (uint32_t)p.vocab);
-            const long o = (long)g * p.n + k;
-            p.out_scores[o] = (float)v;
-            p.out_parents[o] = r;
-            p.out_tokens[o] = token;
-            p.out_ended[o] = token == p.eos || (p.ended != nullptr && p.ended[(long)g * p.W + r] != 0);
+            beam_out(p, g, k, v, index);
             at[list] += 1;
             mine();
         }
@@ -295,18 +381,17 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(ReorderParams p) {
 using namespace smh;
 
 namespace {
-struct SelectPlan { int slices, width; size_t sums, maxima, cands, bytes, fixed, lists; };
-// Slices of 32768 columns where there are rows to fill the GPU with, of 8192 else (the second launch is short where lists are few)
-SelectPlan select_plan(long rows, int W, int vocab, int n) {
+struct SelectPlan { int slices, width; size_t sums, maxima, cands, bytes; };
+// Slices of 32768 columns where there are 256 of them, of 8192 else (us a call, wide and narrow slices of 32016 columns, 8 beams a group: 64 rows 19.6 and 18.4, 160 20.0 and 20.4, 320 25.1 and
+// 28.0, 512 26.4 and 32.3, 1600 51 and 62)
+SelectPlan select_plan(long rows, int vocab, int n) {
     SelectPlan p;
-    p.width = rows * ((vocab + 32767) / 32768) >= 384 && vocab > 8192 && n <= 64 ? 32768 : 8192;      // (64: 32 KB of candidates)
+    p.width = rows * ((vocab + 32767) / 32768) >= 256 && vocab > 8192 && n <= 64 ? 32768 : 8192;      // (64: 32 KB of candidates)
     p.slices = (vocab + p.width - 1) / p.width;
     p.sums = (size_t)rows * p.slices * 8;
     p.maxima = ((size_t)rows * p.slices * 4 + 7) / 8 * 8;
     p.cands = (size_t)rows * p.slices * n * 4;
     p.bytes = p.sums + p.maxima + p.cands;
-    p.fixed = (size_t)W * 12 + (size_t)W * p.slices * 4;               // LDS of the second launch, and of all its lists
-    p.lists = (size_t)W * p.slices * n * 4;
     return p;
 }
 bool select_sizes(int G, int W, int vocab, int n) {
@@ -315,7 +400,7 @@ bool select_sizes(int G, int W, int vocab, int n) {
 }  // namespace
 
 extern "C" size_t smh_beam_select_workspace_bytes(int G, int W, int vocab, int n) {
-    return select_sizes(G, W, vocab, n) ? select_plan((long)G * W, W, vocab, n).bytes : 0;
+    return select_sizes(G, W, vocab, n) ? select_plan((long)G * W, vocab, n).bytes : 0;
 }
 
 extern "C" int smh_beam_select(const void *logits, long ld, const float *scores, const uint8_t *ended, int G, int W, int vocab, int n, int64_t eos, float *out_scores,
@@ -326,12 +411,11 @@ extern "C" int smh_beam_select(const void *logits, long ld, const float *scores,
     SMH_REQUIRE(ld >= vocab, "smh_beam_select: ld=%ld below vocab=%d", ld, vocab);
     SMH_REQUIRE(eos >= 0 && eos < vocab, "smh_beam_select: eos=%ld outside the vocabulary of %d", (long)eos, vocab);
     SMH_REQUIRE(logits && scores && out_scores && out_parents && out_tokens && out_ended, "smh_beam_select: null pointer");
-    const SelectPlan plan = select_plan((long)G * W, W, vocab, n);
+    const SelectPlan plan = select_plan((long)G * W, vocab, n);
     SMH_REQUIRE(W * plan.slices <= BEAM_MAX_LISTS, "smh_beam_select: W=%d beams x %d slices of the vocabulary (at most %d)", W, plan.slices, BEAM_MAX_LISTS);
     SMH_REQUIRE(workspace && ((uintptr_t)workspace & 7) == 0 && workspace_bytes >= plan.bytes, "smh_beam_select: workspace of %zu bytes, %zu needed (8-byte aligned)", workspace_bytes, plan.bytes);
     char *ws = (char *)workspace;
-    const bool held = plan.fixed + plan.lists <= 65536;
-    SelectParams p{(const half_t *)logits, ld, scores, ended, G * W, W, G, vocab, n, (int)eos, plan.slices, plan.width, held,
+    SelectParams p{(const half_t *)logits, ld, scores, ended, G * W, W, G, vocab, n, (int)eos, plan.slices, plan.width,
                    (float *)(ws + plan.sums), (double *)ws, (uint32_t *)(ws + plan.sums + plan.maxima), out_scores, out_parents, out_tokens, out_ended};
     const hipStream_t st = (hipStream_t)stream;
     // (rows along y: at most 65535 a launch)
@@ -348,7 +432,11 @@ extern "C" int smh_beam_select(const void *logits, long ld, const float *scores,
         else hipLaunchKernelGGL(beam_slice_kernel<4>, dim3(plan.slices, rows), dim3(256), n * 128, st, part);
         if (int rc = launch_status()) return rc;
     }
-    hipLaunchKernelGGL(beam_merge_kernel, dim3(G), dim3(64), plan.fixed + (held ? plan.lists : 0), st, p);
+    const long all = (long)W * plan.slices * n;
+    if (all <= 256) hipLaunchKernelGGL((beam_pick_kernel<4, 1>), dim3(G), dim3(64), 0, st, p);
+    else if (all <= 1024) hipLaunchKernelGGL((beam_pick_kernel<4, 4>), dim3(G), dim3(256), 0, st, p);
+    else if (all <= 8192) hipLaunchKernelGGL((beam_pick_kernel<8, 16>), dim3(G), dim3(1024), 0, st, p);
+    else hipLaunchKernelGGL(beam_merge_kernel, dim3(G), dim3(64), (size_t)W * plan.slices * 4, st, p);
     return launch_status();
 }
 
