@@ -530,7 +530,7 @@ int smh_kv8_rows(void *out_k, void *out_v, int B, int Hkv, int D, const int32_t 
 
 /* ---- beam search ---------------------------------------------------------------------------------------------------------
  * The other search next to the tree sampler (the reference has only the latter, mcts.py:67-182).
- * smh_beam_select    G groups of W beams, W <= 64: of all continuations (beam r, token t) of a group the n <= 128 with the largest
+ * smh_beam_select    G groups of W beams, W <= 64: of all W * vocab continuations (beam r, token t) of a group the n <= 128 with the largest
  *                    scores[r] + x[r, t] - log(sum over t' of exp(x[r, t'])), in descending order, equal ones by (r, t).  logits fp16 [G * W, ld], scores fp32 [G * W], out_scores
  *                    fp32, out_parents int32 (r within the group), out_tokens int64, out_ended uint8 [G, n].  ended uint8 [G * W] or NULL: an ended beam has one
  *                    continuation, eos, with its score unchanged; out_ended: the beam had ended or the token is eos.  A logit of -infinity forbids a token (one of +infinity counts as 65536), a score of

@@ -395,7 +395,7 @@ SelectPlan select_plan(long rows, int vocab, int n) {
     return p;
 }
 bool select_sizes(int G, int W, int vocab, int n) {
-    return G >= 1 && W >= 1 && W <= BEAM_MAX_W && vocab >= 1 && vocab <= (1 << 24) && n >= 1 && n <= BEAM_MAX_N && n <= vocab && (long)G * W <= (1 << 20);
+    return G >= 1 && W >= 1 && W <= BEAM_MAX_W && vocab >= 1 && vocab <= (1 << 24) && n >= 1 && n <= BEAM_MAX_N && n <= (long)W * vocab && (long)G * W <= (1 << 20);
 }
 }  // namespace
 
@@ -406,7 +406,7 @@ extern "C" size_t smh_beam_select_workspace_bytes(int G, int W, int vocab, int n
 extern "C" int smh_beam_select(const void *logits, long ld, const float *scores, const uint8_t *ended, int G, int W, int vocab, int n, int64_t eos, float *out_scores,
                                int32_t *out_parents, int64_t *out_tokens, uint8_t *out_ended, void *workspace, size_t workspace_bytes, smh_stream_t stream) {
     SMH_REQUIRE(W >= 1 && W <= BEAM_MAX_W, "smh_beam_select: W=%d (1 .. %d beams a group)", W, BEAM_MAX_W);
-    SMH_REQUIRE(n >= 1 && n <= BEAM_MAX_N && n <= vocab, "smh_beam_select: n=%d of vocab=%d (1 .. %d, at most the vocabulary)", n, vocab, BEAM_MAX_N);
+    SMH_REQUIRE(n >= 1 && n <= BEAM_MAX_N && n <= (long)W * vocab, "smh_beam_select: n=%d of %d beams x vocab=%d (1 .. %d)", n, W, vocab, BEAM_MAX_N);
     SMH_REQUIRE(select_sizes(G, W, vocab, n), "smh_beam_select: G=%d W=%d vocab=%d", G, W, vocab);
     SMH_REQUIRE(ld >= vocab, "smh_beam_select: ld=%ld below vocab=%d", ld, vocab);
     SMH_REQUIRE(eos >= 0 && eos < vocab, "smh_beam_select: eos=%ld outside the vocabulary of %d", (long)eos, vocab);
@@ -458,8 +458,8 @@ extern "C" int smh_beam_reorder(const int32_t *parents, int G, int W, int n, voi
         SMH_REQUIRE(units[i] == 0 || upto, "smh_beam_reorder: tensor %d goes by *upto, which is null", i);
         for (int j = 0; j < i; ++j) SMH_REQUIRE(tensors[i] != tensors[j], "smh_beam_reorder: tensors %d and %d are the same", j, i);
     }
-    // a strip of a group is at most 64 KB of LDS: 256 pieces of 16 bytes up to 16 beams, 64 of 64
-    p.pieces_log2 = W <= 16 ? 8 : W <= 32 ? 7 : 6;
+    // a strip of a group is at most 32 KB of LDS: 256 pieces of 16 bytes up to 8 beams, 32 of 64
+    p.pieces_log2 = W <= 8 ? 8 : W <= 16 ? 7 : W <= 32 ? 6 : 5;
     long strips = 0;
     for (int i = 0; i < n; ++i) {
         p.at[i] = (char *)tensors[i];

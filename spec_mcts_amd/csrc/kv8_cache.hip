@@ -137,6 +137,12 @@ __global__ __launch_bounds__(256) void kv8_append_one_kernel(AppendParams p) {
     const Kv8Seq s = kv8_seq(p.lens, p.cu, b, p.T, 1);
     if (s.n == 0) return;
     const int t = threadIdx.x, c = t & 15, quad = t >> 4, n_rep = p.H / p.Hkv;
+    auto source = [&](int r) {
+        const half_t *x = r == 0 ? p.k + s.t0 * p.k_stride + kvh * KV8_DIM : r == 1 ? p.v + s.t0 * p.v_stride + kvh * KV8_DIM : p.q + s.t0 * p.q_stride + ((long)kvh * n_rep + r - 2) * KV8_DIM;
+        return *reinterpret_cast<const h8 *>(x + c * 8);
+    };
+    h8 x = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (quad < n_rep + 2) x = source(quad);        // (asked for with the sequence's length, not behind it)
     const int at = min(s.old, p.table_rows - 1), row = s.old & 63;
     const half_t *cs = p.cos_tab + (long)at * 64, *sn = p.sin_tab + (long)at * 64;
     const long head = (long)b * p.Hkv + kvh;
@@ -150,22 +156,17 @@ __global__ __launch_bounds__(256) void kv8_append_one_kernel(AppendParams p) {
         open_v_rows(open_v, quad, c, xv);
     }
     for (int r = quad; r < n_rep + 2; r += 16) {
-        if (r == 0) {
-            const h8 x = rope8(*reinterpret_cast<const h8 *>(p.k + s.t0 * p.k_stride + kvh * KV8_DIM + c * 8), cs, sn, c);
-            if (row == 63) fresh[0][c] = x;
-            else if ((s.old >> 6) <= p.c.cols) *reinterpret_cast<h8 *>(open_k + row * KV8_DIM + c * 8) = x;
-        } else if (r == 1) {
-            const h8 x = *reinterpret_cast<const h8 *>(p.v + s.t0 * p.v_stride + kvh * KV8_DIM + c * 8);
-            if (row == 63) fresh[1][c] = x;
-            else if ((s.old >> 6) <= p.c.cols) {
+        if (r >= 16) x = source(r);
+        if (r != 1) x = rope8(x, cs, sn, c);
+        if (r >= 2) *reinterpret_cast<h8 *>(p.q_out + ((long)s.t0 * p.H + (long)kvh * n_rep + r - 2) * KV8_DIM + c * 8) = x;
+        else if (row == 63) fresh[r][c] = x;
+        else if ((s.old >> 6) <= p.c.cols) {
+            if (r == 0) *reinterpret_cast<h8 *>(open_k + row * KV8_DIM + c * 8) = x;
+            else {
                 half_t *at_v = open_v + kv8_place(row);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) at_v[(c * 8 + e) * KV8_ROWS] = x[e];
             }
-        } else {
-            const long h = (long)kvh * n_rep + r - 2;
-            const h8 x = *reinterpret_cast<const h8 *>(p.q + s.t0 * p.q_stride + h * KV8_DIM + c * 8);
-            *reinterpret_cast<h8 *>(p.q_out + ((long)s.t0 * p.H + h) * KV8_DIM + c * 8) = rope8(x, cs, sn, c);
         }
     }
     if (page < 0) return;

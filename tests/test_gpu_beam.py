@@ -54,7 +54,7 @@ def logits_of(rows, vocab, seed, spread=2.0):
     return (torch.randn((rows, vocab), generator=torch.Generator().manual_seed(seed)) * spread).half()
 
 
-@pytest.mark.parametrize("G,W,n,vocab", [(1, 1, 1, 1), (1, 1, 3, 3), (2, 3, 5, 7), (3, 1, 4, 100), (1, 4, 4, 2047), (2, 4, 8, 2048), (1, 5, 5, 2049), (1, 4, 8, 32016), (2, 64, 128, 300),
+@pytest.mark.parametrize("G,W,n,vocab", [(1, 1, 1, 1), (1, 1, 3, 3), (2, 3, 5, 7), (3, 1, 4, 100), (1, 4, 4, 2047), (2, 4, 8, 2048), (1, 5, 5, 2049), (1, 4, 8, 32016), (2, 64, 128, 300), (3, 6, 18, 3), (2, 40, 80, 2),
                                          (1, 64, 64, 32016), (70, 8, 16, 2500), (600, 1, 2, 130), (9, 60, 7, 8193), (1, 2, 128, 129280), (130, 4, 4, 8191)])
 @pytest.mark.parametrize("ended", [False, True])
 def test_sizes(G, W, n, vocab, ended):
@@ -62,6 +62,20 @@ def test_sizes(G, W, n, vocab, ended):
     scores = -torch.rand(G * W, generator=g) * 9
     done = (torch.rand(G * W, generator=g) < 0.3).to(torch.uint8) if ended else None
     check(logits_of(G * W, vocab, vocab), scores, W, n, done, eos=min(EOS, vocab - 1))
+
+
+def test_more_rows_than_a_grid_has():
+    check(logits_of(70000, 9, 3), -torch.rand(70000, generator=torch.Generator().manual_seed(3)), 1, 3)
+    check(logits_of(70000, 9, 4), -torch.rand(70000, generator=torch.Generator().manual_seed(4)), 10, 12)
+
+
+@pytest.mark.parametrize("W,n,vocab", [(4, 64, 32016), (8, 32, 32016), (8, 33, 32016), (32, 64, 32016), (33, 64, 32016), (64, 128, 8192), (64, 128, 8193)])
+def test_every_way_to_pick(W, n, vocab):
+    """candidates for one wave, four, sixteen, and more of them than that; equal ones among them"""
+    x = logits_of(W, vocab, W + n)
+    check(x, -torch.rand(W, generator=torch.Generator().manual_seed(n)), W, n)
+    check((x * 2).round() / 2, torch.zeros(W), W, n)
+    check(x[:1].expand(W, -1).contiguous(), torch.zeros(W), W, n)
 
 
 def test_first_step():
@@ -172,7 +186,7 @@ def moved(x, parents, cols=None):
     return y
 
 
-@pytest.mark.parametrize("G,W", [(1, 1), (1, 2), (3, 4), (2, 64), (17, 5)])
+@pytest.mark.parametrize("G,W", [(1, 1), (1, 2), (3, 4), (2, 64), (17, 5), (4, 8), (2, 9), (2, 16), (1, 17), (1, 33)])
 @pytest.mark.parametrize("upto", [0, 1, 33, 1000, 2 ** 31 - 1, -5])
 def test_states_follow(G, W, upto):
     g = torch.Generator(device=DEV).manual_seed(G * W)

@@ -343,6 +343,20 @@ def test_tables_wider_than_the_batch_and_strided_queries():
     w.check_attn(q, [1] * 4, cu)
 
 
+def test_outputs_over_the_queries():
+    """q rotated and the attention in place of the queries"""
+    for new, max_len in (([1, 1], 512), ([1, 1], 64), ([9, 3], 512), ([150, 40], 512)):
+        w = World(2, 8, 2, 512, seed=29)
+        w.step([200, 77])
+        q, k, v = w.rows(sum(new))
+        ref, _, cu = w.step(new, qkv=(q, k, v), advance=False)
+        mine = q.to(DEV)
+        K().kv8_append(mine, k.to(DEV), v.to(DEV), w.cos_d, w.sin_d, w.cache, w.before, cu=cu, max_new=max(new), out=mine)
+        assert torch.equal(mine, ref)
+        want = K().kv8_attn(ref, w.cache, w.before, cu=cu, max_new=max(new), max_len=max_len)
+        assert torch.equal(K().kv8_attn(mine, w.cache, w.before, cu=cu, max_new=max(new), max_len=max_len, out=mine), want)
+
+
 def test_a_nan_query_has_a_nan_output():
     w = World(1, 2, 1, 4096, seed=25)
     w.step([3000])

@@ -171,11 +171,11 @@ def test_workspaces():
     # a window keeps a long sequence from being cut into more parts than it shows
     assert lib.smh_kv8_attn_workspace_bytes(1, 1, 32, 32, 1, 10 ** 6, 64, 4) < lib.smh_kv8_attn_workspace_bytes(1, 1, 32, 32, 1, 10 ** 6, 0, 0)
     assert lib.smh_beam_select_workspace_bytes(1, 4, 32016, 8) > 4 * 8 * 4
-    for bad in ((0, 4, 100, 4), (1, 65, 100, 4), (1, 0, 100, 4), (1, 4, 100, 129), (1, 4, 3, 4), (1 << 20, 2, 100, 4)):
+    for bad in ((0, 4, 100, 4), (1, 65, 100, 4), (1, 0, 100, 4), (1, 4, 100, 129), (1, 4, 3, 13), (1 << 20, 2, 100, 4)):
         assert lib.smh_beam_select_workspace_bytes(*bad) == 0
 
 
-@pytest.mark.parametrize("bad,why", [(dict(W=65), b"beams"), (dict(W=0), b"beams"), (dict(n=0), b"n="), (dict(n=129), b"n="), (dict(n=100, vocab=99, ld=99), b"n="), (dict(G=0), b"G="),
+@pytest.mark.parametrize("bad,why", [(dict(W=65), b"beams"), (dict(W=0), b"beams"), (dict(n=0), b"n="), (dict(n=129), b"n="), (dict(n=100, W=2, vocab=49, ld=50), b"n="), (dict(G=0), b"G="),
                                      (dict(ld=40), b"ld="), (dict(eos=-1), b"eos"), (dict(eos=50), b"eos"), (dict(logits=None), b"null"), (dict(ws=None), b"workspace"),
                                      (dict(ws_bytes=8), b"workspace"), (dict(ws=(1 << 20) + 4), b"workspace"), (dict(W=64, vocab=1 << 24, ld=1 << 24), b"slices")], ids=str)
 def test_c_select_refuses(bad, why):
