@@ -6,7 +6,7 @@
 // ended when just n are left above).
 //   Order: within a row the fp16 values order exactly; between rows the scores are compared in 64 bits, with sums in 64 bits of fp32 terms, so that
 //   candidates keep their order unless they are closer than the terms' roundings (2^-24 each) leave the sums.
-// Bound: 2 bytes a logit from HBM; short of that by the exponentials and their 64-bit sums (512 rows of 32016: 18 us for the first launch, of which HBM needs 6.6) and, for few rows, by
+// Bound: 2 bytes a logit from HBM; short of that by the exponentials and their 64-bit sums (512 rows of 32016: 17 us for the first launch, of which HBM needs 6.6) and, for few rows, by
 // two launches (4 rows: 6.6 and 5.0 us).
 //
 // Reordering.  Row i of a group takes the contents of row parents[i], in place: a workgroup owns a strip of all rows of a group, has it in LDS and then writes.
@@ -382,11 +382,11 @@ using namespace smh;
 
 namespace {
 struct SelectPlan { int slices, width; size_t sums, maxima, cands, bytes; };
-// Slices of 32768 columns where there are 256 of them, of 8192 else (us a call, wide and narrow slices of 32016 columns, 8 beams a group: 64 rows 19.6 and 18.4, 160 20.0 and 20.4, 320 25.1 and
-// 28.0, 512 26.4 and 32.3, 1600 51 and 62)
+// Slices of 16384 columns where there are 512 of them, of 8192 else (us a call, wide and narrow slices of 32016 columns, 8 beams a group: 64 rows 19.6 and 18.4, 160 20.7 and 20.4, 320 23.8 and
+// 28.0, 512 26.7 and 32.3, 1600 48.8 and 62; slices of 32768: 24.9, 26.7 and 50.7 for the last three)
 SelectPlan select_plan(long rows, int vocab, int n) {
     SelectPlan p;
-    p.width = rows * ((vocab + 32767) / 32768) >= 256 && vocab > 8192 && n <= 64 ? 32768 : 8192;      // (64: 32 KB of candidates)
+    p.width = rows * ((vocab + 16383) / 16384) >= 512 && vocab > 8192 ? 16384 : 8192;
     p.slices = (vocab + p.width - 1) / p.width;
     p.sums = (size_t)rows * p.slices * 8;
     p.maxima = ((size_t)rows * p.slices * 4 + 7) / 8 * 8;
@@ -428,7 +428,7 @@ extern "C" int smh_beam_select(const void *logits, long ld, const float *scores,
         part.slice_sum += (long)r * plan.slices;
         part.cand += (long)r * plan.slices * n;
         const int rows = min(65535, G * W - r);
-        if (plan.width == 32768) hipLaunchKernelGGL(beam_slice_kernel<16>, dim3(plan.slices, rows), dim3(256), n * 512, st, part);
+        if (plan.width == 16384) hipLaunchKernelGGL(beam_slice_kernel<8>, dim3(plan.slices, rows), dim3(256), n * 256, st, part);
         else hipLaunchKernelGGL(beam_slice_kernel<4>, dim3(plan.slices, rows), dim3(256), n * 128, st, part);
         if (int rc = launch_status()) return rc;
     }
