@@ -637,13 +637,16 @@ PyObject *beam_select(Args x) {
     }
     const long eos = whole_number(x[5]);
     here.check();
+    const int g = small(G, "too many groups"), w = small(W, "too many beams"), vo = small(vocab, "the vocabulary is too large"), m = small(n, "n is too large");
+    const size_t bytes = G > 0 ? api.beam_select_bytes(g, w, vo, m) : 0;
+    const long ld = rows <= 1 ? vocab : logits.stride(0);
+    if (G > 0 && bytes == 0)                       // (sizes that it refuses, with its reason; nothing of that size is allocated)
+        check(api.beam_select(nullptr, ld, nullptr, nullptr, g, w, vo, m, eos, nullptr, nullptr, nullptr, nullptr, nullptr, 0, stream()), "smh_beam_select");
     at::Tensor best = empty({G, n}, at::kFloat, logits), parents = empty({G, n}, at::kInt, logits), tokens = empty({G, n}, at::kLong, logits), done = empty({G, n}, at::kByte, logits);
     if (G > 0) {
-        const int g = small(G, "too many groups"), w = small(W, "too many beams"), vo = small(vocab, "the vocabulary is too large"), m = small(n, "n is too large");
-        const size_t bytes = api.beam_select_bytes(g, w, vo, m);
         at::Tensor ws = empty({(int64_t)bytes}, at::kByte, logits);
-        check(api.beam_select(logits.data_ptr(), rows <= 1 ? vocab : logits.stride(0), scores.data_ptr<float>(), ended ? (const uint8_t *)ended->data_ptr() : nullptr, g, w, vo, m, eos,
-                              best.data_ptr<float>(), parents.data_ptr<int32_t>(), tokens.data_ptr<int64_t>(), done.data_ptr<uint8_t>(), bytes ? ws.data_ptr() : nullptr, bytes, stream()),
+        check(api.beam_select(logits.data_ptr(), ld, scores.data_ptr<float>(), ended ? (const uint8_t *)ended->data_ptr() : nullptr, g, w, vo, m, eos, best.data_ptr<float>(),
+                              parents.data_ptr<int32_t>(), tokens.data_ptr<int64_t>(), done.data_ptr<uint8_t>(), ws.data_ptr(), bytes, stream()),
               "smh_beam_select");
     }
     return made(Py_BuildValue("(NNNN)", give(best), give(parents), give(tokens), give(done)));

@@ -151,6 +151,14 @@ def test_defaults_and_empty():
     assert K().beam_select(x[:0], s[:0], 3)[2].shape == (0, 3)
 
 
+@pytest.mark.parametrize("kw,why", [(dict(beams=65), "beams"), (dict(n=129), "n="), (dict(n=10 ** 9), "n="), (dict(eos=100), "eos"), (dict(eos=-1), "eos")], ids=str)
+def test_sizes_that_are_refused(kw, why):
+    from spec_mcts_amd._lib import SmhError
+    x, s = logits_of(65, 100, 8).to(DEV), torch.zeros(65, device=DEV)
+    with pytest.raises(SmhError, match=why):
+        K().beam_select(x, s, **{**dict(beams=13, n=5), **kw})
+
+
 def test_captured_and_on_two_streams():
     x, s = logits_of(8, 32016, 9).to(DEV), torch.linspace(-2, 0, 8, device=DEV)
     want = [K().beam_select(x.roll(i, 0).contiguous(), s, 4) for i in range(4)]
