@@ -148,19 +148,34 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(SelectParams p) {
 }
 
 // What the second launch knows of a row
-struct BeamRow { double base; float max; };        // score - log sum (of an ended beam the score); the largest logit, NaN: the row's candidates go by index
+struct BeamRow { double base; float max; int ended; };      // score - log sum (of an ended beam the score); the largest logit, NaN: the row's candidates go by index
 __device__ __forceinline__ BeamRow beam_row(const SelectParams &p, long row) {
+    // everything is asked for at once: what the first launch left of an ended or lost beam is not used
     const float score = p.scores[row];
-    if (!(score > -INFINITY) || (p.ended != nullptr && p.ended[row] != 0)) return BeamRow{(double)score, __builtin_nanf("")};
+    const int ended = p.ended != nullptr && p.ended[row] != 0;
     float m = -INFINITY;
     double s = 0.0;
-    for (int i = 0; i < p.slices; ++i) m = fmaxf(m, p.slice_max[row * p.slices + i]);
-    for (int i = 0; i < p.slices; ++i) {
-        const float mi = p.slice_max[row * p.slices + i];
-        s += p.slice_sum[row * p.slices + i] * (mi == m ? 1.0 : exp((double)mi - (double)m));
+    for (int i0 = 0; i0 < p.slices; i0 += 4) {
+        float mi[4];
+        double si[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const long at = row * p.slices + min(i0 + i, p.slices - 1);
+            mi[i] = p.slice_max[at];
+            si[i] = p.slice_sum[at];
+        }
+        float now = m;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) now = fmaxf(now, mi[i]);
+        if (m != now) s *= m == -INFINITY ? 0.0 : exp((double)m - (double)now);
+        m = now;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i0 + i < p.slices) s += si[i] * (mi[i] == m ? 1.0 : exp((double)mi[i] - (double)m));
     }
+    if (!(score > -INFINITY) || ended) return BeamRow{(double)score, __builtin_nanf(""), ended};
     // (36 bits of the sum: rows of the same values in another order are equal)
-    return BeamRow{(double)score - log(__longlong_as_double((__double_as_longlong(s) + (1 << 15)) & ~0xFFFFll)), m};
+    return BeamRow{(double)score - log(__longlong_as_double((__double_as_longlong(s) + (1 << 15)) & ~0xFFFFll)), m, 0};
 }
 constexpr uint32_t BEAM_NONE = 0xFFFFFFFFu;        // (beam * vocab + token is below 2^30)
 // Candidate i of list (row r, slice) with its key: score and index; BEAM_NONE: there is none
@@ -182,13 +197,13 @@ __device__ __forceinline__ void beam_candidate(const SelectParams &p, const Beam
     const float v = beam_value(key >> 16);
     if (v > -INFINITY) value = row.base + ((double)v - (double)row.max);
 }
-__device__ __forceinline__ void beam_out(const SelectParams &p, int g, int k, double value, uint32_t index) {
+__device__ __forceinline__ void beam_out(const SelectParams &p, const BeamRow *rows, int g, int k, double value, uint32_t index) {
     const int r = (int)(index / (uint32_t)p.vocab), token = (int)(index - (uint32_t)r * (uint32_t)p.vocab);
     const long o = (long)g * p.n + k;
     p.out_scores[o] = (float)value;
     p.out_parents[o] = r;
     p.out_tokens[o] = token;
-    p.out_ended[o] = token == p.eos || (p.ended != nullptr && p.ended[(long)g * p.W + r] != 0);
+    p.out_ended[o] = token == p.eos || rows[r].ended;
 }
 // 64 bits that order as the numbers do
 __device__ __forceinline__ uint64_t ordered64(double v) {
@@ -268,7 +283,7 @@ __global__ __launch_bounds__(64 * WAVES) void beam_pick_kernel(SelectParams p) {
         const uint32_t x = best_index[i];
         int above = 0;
         for (int j = 0; j < found; ++j) above += best[j] > s || (best[j] == s && best_index[j] < x);
-        beam_out(p, g, above, unordered64(s), x);
+        beam_out(p, rows, g, above, unordered64(s), x);
     }
 }
 
@@ -315,7 +330,7 @@ __global__ __launch_bounds__(64) void beam_merge_kernel(SelectParams p) {
             lane_of = __ffsll((unsigned long long)__ballot(index == x)) - 1;
         }
         if (lane == lane_of) {
-            beam_out(p, g, k, v, index);
+            beam_out(p, rows, g, k, v, index);
             at[list] += 1;
             mine();
         }
@@ -432,10 +447,12 @@ extern "C" int smh_beam_select(const void *logits, long ld, const float *scores,
         else hipLaunchKernelGGL(beam_slice_kernel<4>, dim3(plan.slices, rows), dim3(256), n * 128, st, part);
         if (int rc = launch_status()) return rc;
     }
+    // (us a call of 32016 columns: 64 beams, 128 kept, 65, by the merge 253; 32 beams, 64 kept, 34 and 87)
     const long all = (long)W * plan.slices * n;
     if (all <= 256) hipLaunchKernelGGL((beam_pick_kernel<4, 1>), dim3(G), dim3(64), 0, st, p);
     else if (all <= 1024) hipLaunchKernelGGL((beam_pick_kernel<4, 4>), dim3(G), dim3(256), 0, st, p);
     else if (all <= 8192) hipLaunchKernelGGL((beam_pick_kernel<8, 16>), dim3(G), dim3(1024), 0, st, p);
+    else if (all <= 32768) hipLaunchKernelGGL((beam_pick_kernel<32, 16>), dim3(G), dim3(1024), 0, st, p);
     else hipLaunchKernelGGL(beam_merge_kernel, dim3(G), dim3(64), (size_t)W * plan.slices * 4, st, p);
     return launch_status();
 }

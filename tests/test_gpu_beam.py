@@ -69,7 +69,7 @@ def test_more_rows_than_a_grid_has():
     check(logits_of(70000, 9, 4), -torch.rand(70000, generator=torch.Generator().manual_seed(4)), 10, 12)
 
 
-@pytest.mark.parametrize("W,n,vocab", [(4, 64, 32016), (8, 32, 32016), (8, 33, 32016), (32, 64, 32016), (33, 64, 32016), (64, 128, 8192), (64, 128, 8193)])
+@pytest.mark.parametrize("W,n,vocab", [(4, 64, 32016), (8, 32, 32016), (8, 33, 32016), (32, 64, 32016), (33, 64, 32016), (64, 128, 8192), (64, 128, 8193), (64, 128, 32768), (64, 128, 32769)])
 def test_every_way_to_pick(W, n, vocab):
     """candidates for one wave, four, sixteen, and more of them than that; equal ones among them"""
     x = logits_of(W, vocab, W + n)
