@@ -536,7 +536,8 @@ long kv8_blocks(int max_new, long max_len, int window, int sinks) {
 // 12 of 8000, four tokens, 39 / 42 / 48 / 55; one of 4095, 32 heads, 13 each; with 256: 113, 46, 14.
 // With 128 workgroups and more without parts those are of eight blocks at least (512 new tokens, 64 heads over 8, one part or two: 27 and 36 us; 300 new ones of two heads behind 5000
 // rows, which are few workgroups, 26 and 21 with eight and four blocks).
-// Up to 12 blocks a sequence are one part, without a second launch (one token of 32 heads, us in parts and in one: 512 rows 10.7 and 6.9, 701 rows 11.1 and 9.5, 1001 rows 10.5 and 11.1).
+// Up to 12 blocks a sequence are one part, without a second launch (one token of 32 heads, us in parts and in one: 512 rows 10.7 and 6.9, 701 rows 11.1 and 9.5, 1001 rows 10.5 and 11.1), with
+// 128 workgroups and more up to 40 (8 such sequences of 1500 and 2400 rows 22.1 and 19.8, 28.3 and 25.1; 20 of 64 heads over 8 17.7 and 16.0, 21.5 and 21.3).
 // 33 .. 64 queries: tiles of one wave each over shared codes (3 x 130000 rows, five tokens of 8 queries, 140 us; three tiles in a wave, one wave a SIMD, 144; two waves a block, two tiles
 // each, 161).  Up to 32 queries waves of their own: four tokens 123 and 138 us.  64 queries a workgroup, four of which run at a time, also where the sequences are short: 500 tokens of 32
 // heads 19.7 us, 22.7 with 128 queries, 512 of 64 over 8 22.9 and 27.2; 2000 of 64 over 8 100 and 96.
@@ -548,7 +549,7 @@ Kv8Plan kv8_plan(int B, int H, int Hkv, int max_new, long max_len, int window, i
     p.groups = p.tiles ? 1 : (rows + p.rows - 1) / p.rows;
     const long base = (long)B * Hkv * p.groups, want = (p.tiles || p.rows == 128 ? 512 : 1024) / base, most = blocks / (base < 128 ? 4 : 8);
     long s = want < most ? want : most;
-    if (p.tiles && blocks <= 12) s = 1;
+    if (p.tiles && blocks <= (base >= 128 ? 40 : 12)) s = 1;
     p.splits = (int)(s < 1 ? 1 : s > KV8_MAX_SPLITS ? KV8_MAX_SPLITS : s);
     return p;
 }
