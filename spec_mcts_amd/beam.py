@@ -26,7 +26,7 @@ class BeamSearch:
     def _buffers(self, dev, steps: int) -> None:
         W = self.beams
         self._fwd = BucketedForward(self.model, W, use_graph=self.use_graph)
-        self._key = (steps, self.eos, self.use_graph, dev)
+        self._key = (W, steps, self.eos, self.use_graph, dev)
         self.results = torch.zeros((W, steps), dtype=torch.int64, device=dev)
         self.scores = torch.zeros(W, dtype=torch.float32, device=dev)
         self.ended = torch.zeros(W, dtype=torch.uint8, device=dev)
@@ -56,7 +56,7 @@ class BeamSearch:
         dev = m.norm.weight.device
         assert prompt.shape[1] <= m.params.max_prompt_seq_len
         steps = min(self.max_new, m.params.max_seq_len)
-        if self._fwd is None or self._key != (steps, self.eos, self.use_graph, dev) or self._fwd.model is not m:
+        if self._fwd is None or self._key != (W, steps, self.eos, self.use_graph, dev) or self._fwd.model is not m:
             self._buffers(dev, steps)
         fwd = self._fwd
         m.resetSeq()

@@ -569,7 +569,7 @@ extern "C" int smh_kv8_attn(const void *q, void *out, int T, int B, int H, int H
     SMH_REQUIRE(B >= 1 && B <= 65535 && Hkv >= 1 && Hkv <= 4096 && H >= Hkv && H % Hkv == 0 && H <= 65535, "smh_kv8_attn: B=%d (1 .. 65535) H=%d Hkv=%d (1 .. 4096)", B, H, Hkv);
     SMH_REQUIRE(T >= 0 && max_new >= 0 && max_new <= KV8_MAX_LEN && max_len >= 1 && window >= 0 && window <= KV8_MAX_LEN && sinks >= 0 && sinks <= KV8_MAX_LEN,
                 "smh_kv8_attn: T=%d max_new=%d max_len=%ld window=%d sinks=%d", T, max_new, max_len, window, sinks);
-    SMH_REQUIRE(cu || T == B, "smh_kv8_attn: without cu every sequence has one row: T=%d B=%d", T, B);
+    SMH_REQUIRE(cu || (T == B && max_new == 1), "smh_kv8_attn: without cu every sequence has one row: T=%d B=%d max_new=%d", T, B, max_new);
     SMH_REQUIRE(q_stride >= (long)H * D && q_stride % 8 == 0, "smh_kv8_attn: token stride %ld", q_stride);
     SMH_REQUIRE(codes_k && codes_v && scales && open_k && open_v && pages, "smh_kv8_attn: null pointer in the cache");
     SMH_REQUIRE(aligned16(codes_k) && aligned16(codes_v) && aligned16(open_k) && aligned16(open_v) && ((uintptr_t)scales & 7) == 0,

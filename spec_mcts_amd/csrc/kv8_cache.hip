@@ -335,7 +335,7 @@ extern "C" int smh_kv8_append(const void *q, const void *k, const void *v, void 
     if (cache_ok("smh_kv8_append", codes_k, codes_v, scales, open_k, open_v, pages, n_pages, pages_stride, pages_cols, B, Hkv, D)) return -1;
     SMH_REQUIRE(H >= 1 && H % Hkv == 0 && H + Hkv <= 65535, "smh_kv8_append: H=%d Hkv=%d", H, Hkv);
     SMH_REQUIRE(T >= 0 && max_new >= 0 && max_new <= KV8_MAX_LEN && table_rows >= 1, "smh_kv8_append: T=%d max_new=%d table_rows=%d", T, max_new, table_rows);
-    SMH_REQUIRE(cu || T == B, "smh_kv8_append: without cu every sequence has one row: T=%d B=%d", T, B);
+    SMH_REQUIRE(cu || (T == B && max_new == 1), "smh_kv8_append: without cu every sequence has one row: T=%d B=%d max_new=%d", T, B, max_new);
     SMH_REQUIRE(q_stride >= (long)H * D && k_stride >= (long)Hkv * D && v_stride >= (long)Hkv * D && q_stride % 8 == 0 && k_stride % 8 == 0 && v_stride % 8 == 0,
                 "smh_kv8_append: token strides %ld %ld %ld", q_stride, k_stride, v_stride);
     if (T == 0 || max_new == 0) return 0;

@@ -131,6 +131,17 @@ def test_what_is_not_finite():
     check(torch.full((2, 70), -math.inf).half(), torch.full((2,), -math.inf), 2, 70, torch.ones(2, dtype=torch.uint8), eos=0)
 
 
+@pytest.mark.parametrize("infinite", [False, True])
+def test_every_pattern_of_a_logit(infinite):
+    """All values that 16 bits have, quiet and signalling NaN of either sign among them, which count as -infinity"""
+    x = torch.arange(65536, dtype=torch.int32)
+    x = torch.stack([x[torch.randperm(65536, generator=torch.Generator().manual_seed(s))] for s in (1, 2)]).to(torch.int16).view(torch.float16)
+    if not infinite:
+        x = torch.where(x == math.inf, torch.zeros_like(x), x)
+    check(x, torch.tensor([0.0, -0.5]), 2, 128)
+    check(x, torch.tensor([0.0, -0.5]), 1, 128)
+
+
 def test_wide_range_of_scores():
     """sums of scores as long outputs have them, and logits of large magnitude"""
     check(logits_of(8, 32016, 6, 30.0), -torch.rand(8, generator=torch.Generator().manual_seed(6)) * 4000, 4, 8)

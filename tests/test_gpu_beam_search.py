@@ -97,6 +97,23 @@ def test_limits():
         BeamSearch(m, 2, 4).search(torch.zeros((1, 17), dtype=torch.int64, device=DEV))
 
 
+def test_one_search_object_for_everything():
+    """prompts of several lengths, other numbers of beams, and the sampler on the same model in between, by one object"""
+    from spec_mcts_amd.beam import BeamSearch
+    from spec_mcts_amd.mcts import mcts
+    m = small_model(seed=4)
+    search = BeamSearch(m, 4, 10)
+    for W, P in ((4, 9), (4, 16), (6, 9), (3, 9), (4, 9)):
+        prompt = torch.randint(0, 320, (1, P), generator=torch.Generator().manual_seed(P)).to(DEV)
+        want, lengths, scores = by_starting_over(m, prompt, W, 10, 2)
+        search.beams = W
+        for _ in range(2):
+            tokens, n, s = search.search(prompt)
+            assert torch.equal(tokens.cpu()[:, :want.shape[1]], want) and torch.equal(n.cpu().long(), lengths)
+            assert bool(((s.cpu().double() - scores).abs() <= 1e-4).all())
+            mcts(m, 8, top_k=8, temp=1.0).search(prompt, 8)
+
+
 @pytest.mark.parametrize("window,sinks", [(0, 0), (40, 4)])
 def test_beams_over_the_8_bit_cache(window, sinks):
     """Append, attend, project, select, reorder - one layer over random weights, two prompts of different lengths with three beams each - for 70 steps, past a

@@ -204,3 +204,9 @@ def test_an_empty_cache():
     for bad in (dict(batch=0), dict(max_len=0), dict(n_kv_heads=0), dict(n_pages=0)):
         with pytest.raises(AssertionError):
             K.kv8_cache(**{**dict(batch=1, max_len=1, n_kv_heads=1, device="cpu"), **bad})
+
+
+@pytest.mark.parametrize("max_new", [0, 2, 64])
+def test_one_new_row_without_cu(max_new):
+    assert c_append(max_new=max_new) == -1 and b"without cu" in err()
+    assert c_attn(max_new=max_new) == -1 and b"without cu" in err()
