@@ -435,3 +435,78 @@ def test_offsets_past_32_bits():
     w.check_attn(q, [1], cu)
     k, _ = K().kv8_rows(c, w.lens, torch.zeros_like(w.lens), 251)
     assert torch.equal(k[0].cpu(), w.seqs[0].held()[0].float().half())
+
+
+# ---- blocks whose V differs in size ----------------------------------------------------------------------------------------------
+def scale_world(order, low, rows, H, Hkv, seed):
+    """`rows` rows whose blocks hold V of about 1000 or of 2^low, with one strong row in the first of the large blocks: all others have 2^-11 of its weight, and about as
+    much together.  The tables do not rotate, the scores are the first value's"""
+    w = World(1, H, Hkv, rows + 512, seed=seed)
+    w.cos_d.fill_(1), w.sin_d.fill_(0)
+    w.cos.fill_(1), w.sin.fill_(0)
+    blocks = (rows + 63) // 64
+    large = {"first": [0], "last": [rows // 64 - 1], "middle": [blocks // 2], "turns": range(0, blocks, 2), "zeros": [1]}[order]
+    q, k, v = w.rows(rows)
+    q[:], k[:] = 0, 0
+    q[..., 0] = 1.0
+    k[64 * large[0] + 7, :, 0] = 86.25                          # 86.25 / sqrt(128) = 11 ln 2
+    v = (v.float().abs() * 0.25 + 0.5).half()                   # (one sign: a lost row moves the mean)
+    for j in range(blocks):
+        at = slice(j * 64, j * 64 + 64)
+        v[at] = v[at] * 1000 if j in large else (v[at].float() * 2.0 ** low).half()
+        if order == "zeros" and j % 3 == 2:
+            v[at] = 0
+    w.step([rows], qkv=(q, k, v))
+    return w
+
+
+def check_by_scales(w, q, new, cu, **kw):
+    """As check_attn, with the rounding of the weights counted in the sum that they are divided by too: sum p d (v - o) with |v - o| <= |v| + |o| and |o| below the mean of |v|"""
+    got = K().kv8_attn(q, w.cache, w.before, cu=cu, max_new=max(max(new), 1), **kw).cpu().double()
+    at = 0
+    for b, (s, n) in enumerate(zip(w.seqs, new)):
+        k, v = s.held()
+        o, mean = O.attention(q[at:at + n].cpu(), k, v, k.shape[0] - n, kw.get("window", 0), kw.get("sinks", 0))
+        bound = O.attention_bound(o, mean, k.shape[0], float(v.abs().max())) + 2.0 ** -11 * mean
+        off = (got[at:at + n] - o).abs()
+        assert bool((off <= bound).all()), (b, k.shape[0], kw, float((off / bound).max()))
+        at += n
+
+
+@pytest.mark.parametrize("order", ["first", "last", "middle", "turns", "zeros"])
+@pytest.mark.parametrize("low", [4, -2, -8, -14, -20, -24])
+@pytest.mark.parametrize("new", [1, 9, 150])
+def test_a_block_s_v_does_not_change_what_its_rows_weigh(order, low, new):
+    """large and small V block by block, for few and many queries, in one part and in several"""
+    w = scale_world(order, low, 2500, 4, 2, seed=40 + new)
+    q, k, v = w.rows(new)
+    q[:], k[:] = 0, 0
+    q[..., 0] = 1.0
+    q, _, cu = w.step([new], qkv=(q, k, (v.float() * 2.0 ** low).half()))
+    for kw in (dict(max_len=64), dict(max_len=10 ** 6), dict(window=2000, sinks=100), dict(window=2300, max_len=64)):
+        check_by_scales(w, q, [new], cu, **kw)
+
+
+@pytest.mark.parametrize("new", [[1, 1], [12, 3], [200, 90]], ids=str)
+def test_v_of_any_size_from_block_to_block(new):
+    """random scores over blocks whose V goes from 2^-20 to 2^6, between heads and sequences too"""
+    w = World(2, 6, 2, 2400, seed=43)
+    q, k, v = w.rows(1900 + 801)
+    size = 2.0 ** torch.randint(-20, 7, ((1900 + 801) // 64 + 1, 2), generator=w.g).repeat_interleave(64, 0)[:1900 + 801]
+    w.step([1900, 801], qkv=(q, k, (v.float() * size[..., None]).half()))
+    q, _, cu = w.step(new)
+    for kw in (dict(max_len=64), dict(), dict(max_len=10 ** 6, window=700, sinks=64), dict(max_len=64, window=64)):
+        check_by_scales(w, q, new, cu, **kw)
+
+
+def test_rows_that_are_not_seen_do_not_set_the_unit():
+    """small values in the window behind large ones that it has passed, and in front of large ones that are yet to come"""
+    w = scale_world("middle", -20, 2500, 8, 1, seed=44)
+    q, k, v = w.rows(130)
+    q[:], k[:] = 0, 0
+    q[..., 0] = 1.0
+    v = v.float() * 2.0 ** -20
+    v[70:] *= 2.0 ** 28
+    q, _, cu = w.step([130], qkv=(q, k, v.half()))
+    for max_len in (64, 10 ** 6):
+        check_by_scales(w, q, [130], cu, max_len=max_len, window=300)
