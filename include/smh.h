@@ -506,7 +506,8 @@ int smh_decode_finish(const smh_layer *last, smh_pass *pass, const void *norm_we
  *   pages         int32 [B, pages_stride], pages_cols in use: block j of sequence b is page pages[b, j].  Read ids are cut to 0 .. n_pages - 1; a block whose id
  *                 is outside, or past pages_cols, is not written
  *   lens          int32 [B] on the device: rows of each sequence before the call (the call does not change them).  A sequence has at most
- *                 pages_cols * 64 + 63 rows; what lies past that is neither read nor written
+ *                 pages_cols * 64 + 63 rows; what lies past that is neither read nor written (drafted tokens that run past the end, say: those in front of it are kept).
+ *                 A length, new rows counted, of (pages_cols + 2) * 64 and more is a wrong one: the table's blocks alone are written and read
  *   cu            NULL: one new row for each sequence (T = B, max_new = 1).  Else int32 [B + 1] on the device: the new rows of sequence b are rows cu[b] .. cu[b + 1] - 1 of
  *                 q, k, v (none is fine), of which the first max_new count.  Rows of no sequence are left as they are in the outputs.
  * A row of k or v with an infinity or a NaN makes its block's values of that head NaN (for an open block: those of that row, and the outputs of queries that

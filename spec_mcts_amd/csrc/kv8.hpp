@@ -41,6 +41,12 @@ __device__ __forceinline__ Kv8Seq kv8_seq(const int32_t *lens, const int32_t *cu
     return Kv8Seq{t0, min(t1 - t0, max_new), min(max(lens[b], 0), KV8_MAX_LEN)};
 }
 
+// Rows that a cache keeps of a sequence of `length`: the table's blocks and 63 of the open one behind them.  A length that is 64 and more past these is taken for a wrong one: it
+// has the table's blocks alone.
+__device__ __forceinline__ int kv8_kept(int length, int cols) {
+    return length < (cols + 2) * KV8_ROWS ? min(length, cols * KV8_ROWS + KV8_ROWS - 1) : cols * KV8_ROWS;
+}
+
 // place of row r of a block in a line of V
 __device__ __forceinline__ int kv8_place(int r) { return ((r >> 2) & 3) * 16 + (r >> 5) * 8 + ((r >> 4) & 1) * 4 + (r & 3); }
 

@@ -31,7 +31,7 @@ struct Kv8Span {
 };
 __device__ __forceinline__ Kv8Span kv8_span(const Kv8AttnParams &p, const Kv8Seq &s, int lo, int hi) {      // lo, hi: places of the first and last query
     Kv8Span v;
-    const int total = min(s.old + s.n, p.c.cols * KV8_ROWS + 63);
+    const int total = kv8_kept(s.old + s.n, p.c.cols);
     v.whole = total >> 6;
     v.open_rows = total & 63;
     const int last = min(hi, total - 1) >> 6;

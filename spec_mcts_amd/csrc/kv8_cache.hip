@@ -201,14 +201,13 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendParams p) {
         }
         return;
     }
-    const int kvh = blockIdx.y, total = s.old + s.n, first = s.old >> 6, j = first + blockIdx.x, open = total >> 6;
+    const int kvh = blockIdx.y, total = kv8_kept(s.old + s.n, p.c.cols), first = s.old >> 6, j = first + blockIdx.x, open = total >> 6;
     if (j > open) return;
     const long head = (long)b * p.Hkv + kvh;
     half_t *open_k = p.c.open_k + head * KV8_TILE, *open_v = p.c.open_v + head * KV8_TILE;
     const half_t *k = p.k + (long)s.t0 * p.k_stride + kvh * KV8_DIM, *v = p.v + (long)s.t0 * p.v_stride + kvh * KV8_DIM;
     // the new rows among the total % 64 of the block that stays open
     auto leave_open = [&]() {
-        if (open > p.c.cols) return;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int row = quad * 4 + e, i = open * KV8_ROWS + row - s.old;
@@ -259,7 +258,7 @@ struct RowsParams {
 // Rows as the cache holds them, in fp16: a workgroup has a block and kv head.  Reads 1 (or 2), writes 2 bytes a value.
 __global__ __launch_bounds__(256) void kv8_rows_kernel(RowsParams p) {
     const int kvh = blockIdx.y, b = blockIdx.z, t = threadIdx.x, quad = t >> 4, dc = t & 15;
-    const int first = min(max(p.first[b], 0), KV8_MAX_LEN), total = min(min(max(p.total[b], 0), KV8_MAX_LEN), p.c.cols * KV8_ROWS + 63);
+    const int first = min(max(p.first[b], 0), KV8_MAX_LEN), total = kv8_kept(min(max(p.total[b], 0), KV8_MAX_LEN), p.c.cols);
     const int j = (first >> 6) + blockIdx.x, whole = total >> 6;
     const int row0 = j * KV8_ROWS + quad * 4;
     if (j * KV8_ROWS >= first + p.count) return;

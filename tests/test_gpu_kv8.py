@@ -437,6 +437,60 @@ def test_offsets_past_32_bits():
     assert torch.equal(k[0].cpu(), w.seqs[0].held()[0].float().half())
 
 
+# ---- past the capacity -----------------------------------------------------------------------------------------------------------
+PAST = [(0, 192), (0, 255), (70, 193), (127, 192), (128, 200), (128, 255), (150, 192), (188, 193), (190, 254), (191, 192), (191, 255), (195, 230), (0, 256), (70, 300), (140, 256), (191, 400), (300, 310)]
+
+
+@pytest.mark.parametrize("old,total", PAST, ids=str)
+def test_a_call_past_the_capacity_keeps_the_rows_in_front_of_it(old, total):
+    """a cache of 128 + 63 rows, from `old` rows to `total` in one call and row by row: the same rows, and the attention of the call over them; from 256 on they are those of the table's
+    blocks"""
+    cap = 191 if total < 256 else 128
+    ways = []
+    for one in (True, False):
+        w = World(1, 4, 2, 128, seed=51)
+        w.cos, w.sin = O.tables(512)
+        w.cos_d, w.sin_d = w.cos.to(DEV), w.sin.to(DEV)
+        q, k, v = w.rows(total)
+        qkv = lambda a, b: (q[a:b], k[a:b], v[a:b])             # noqa: E731
+        for i in range(old):
+            w.step([1], qkv=qkv(i, i + 1), single=True)
+        if one:
+            rotated, _, cu = w.step([total - old], qkv=qkv(old, total))
+            out = K().kv8_attn(rotated, w.cache, w.before, cu=cu, max_new=total - old)
+        else:
+            for i in range(old, total):
+                w.step([1], qkv=qkv(i, i + 1), single=True)
+        ways.append((w, K().kv8_rows(w.cache, w.lens, torch.zeros_like(w.lens), total + 70)))
+    w, rows = ways[0]
+    assert all(torch.equal(a, b) for a, b in zip(rows, ways[1][1]))
+    s = w.seqs[0]
+    s.k, s.v = s.k[:cap], s.v[:cap]
+    held = s.held()
+    for got, x in zip(rows, held):
+        assert torch.equal(got[0, :min(cap, total)].cpu(), x.float().half()) and bool((got[0, cap:] == 0).all())
+    for a, b in zip(w.cache[:3], ways[1][0].cache[:3]):
+        assert torch.equal(a[w.cache.pages.long()], b[w.cache.pages.long()])
+    o, mean = O.attention(rotated.cpu(), *held, old)
+    bound = O.attention_bound(o, mean, cap, float(held[1].abs().max()))
+    assert bool(((out.cpu().double() - o).abs() <= bound).all())
+
+
+def test_drafted_tokens_at_the_end():
+    """five drafted tokens of which three have room and are accepted: the next step sees them"""
+    w = World(2, 8, 2, 128, seed=52, places=300)
+    w.step([188, 40])
+    q, k, v = w.rows(10)
+    w.step([5, 5], qkv=(q, k, v), advance=False)
+    w.lens += 3
+    for s in w.seqs:
+        s.k, s.v = s.k[:-2], s.v[:-2]
+    rows = K().kv8_rows(w.cache, w.lens, torch.zeros_like(w.lens), 191)
+    for b, s in enumerate(w.seqs):
+        for got, x in zip(rows, s.held()):
+            assert torch.equal(got[b, :x.shape[0]].cpu(), x.float().half())
+
+
 # ---- blocks whose V differs in size ----------------------------------------------------------------------------------------------
 def scale_world(order, low, rows, H, Hkv, seed):
     """`rows` rows whose blocks hold V of about 1000 or of 2^low, with one strong row in the first of the large blocks: all others have 2^-11 of its weight, and about as
