@@ -117,7 +117,7 @@ struct Kv8Wave {
             float by_scale = scale;
             if (masked) {
                 const int top = min(at[t], limit - 1) - block * KV8_ROWS, low = window > 0 ? at[t] - window - block * KV8_ROWS : -1, first = sinks - block * KV8_ROWS;
-                seen[t] = top >= 0 && (low < 63 || first > 0);
+                seen[t] = top >= 0 && (low < min(top, KV8_ROWS - 1) || first > 0);
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
 #pragma unroll

@@ -491,6 +491,20 @@ def test_drafted_tokens_at_the_end():
             assert torch.equal(got[b, :x.shape[0]].cpu(), x.float().half())
 
 
+@pytest.mark.parametrize("window,sinks,sees", [(62, 0, False), (63, 0, False), (64, 0, True), (63, 128, False), (63, 129, True)])
+def test_a_query_past_the_capacity_sees_what_its_window_shows(window, sinks, sees):
+    """rows 128 .. 190 of a cache of 191, the last of them not finite, and a query at place 253: a window of 63 ends behind them"""
+    w = World(1, 2, 1, 128, seed=53, places=300)
+    q, k, v = w.rows(254)
+    v[190] = math.nan
+    w.step([253], qkv=(q[:253], k[:253], v[:253]))
+    rotated, _, _ = w.step([1], qkv=(q[253:], k[253:], v[253:]), single=True)
+    o = K().kv8_attn(rotated, w.cache, w.before, window=window, sinks=sinks).cpu()
+    assert bool(torch.isnan(o).all()) if sees else bool(torch.isfinite(o).all())
+    if sinks == 0 and not sees:
+        assert bool((o == 0).all())                             # nothing in sight
+
+
 # ---- blocks whose V differs in size ----------------------------------------------------------------------------------------------
 def scale_world(order, low, rows, H, Hkv, seed):
     """`rows` rows whose blocks hold V of about 1000 or of 2^low, with one strong row in the first of the large blocks: all others have 2^-11 of its weight, and about as
