@@ -535,7 +535,8 @@ int smh_kv8_rows(void *out_k, void *out_v, int B, int Hkv, int D, const int32_t 
  *                    scores[r] + x[r, t] - log(sum over t' of exp(x[r, t'])), in descending order, equal ones by (r, t).  logits fp16 [G * W, ld], scores fp32 [G * W], out_scores
  *                    fp32, out_parents int32 (r within the group), out_tokens int64, out_ended uint8 [G, n].  ended uint8 [G * W] or NULL: an ended beam has one
  *                    continuation, eos, with its score unchanged; out_ended: the beam had ended or the token is eos.  A logit of -infinity forbids a token (one of +infinity counts as 65536), a score of
- *                    -infinity a beam (NaN counts as that): their continuations come last, by (r, t).  Compared in 64 bits on sums of fp32 terms.
+ *                    -infinity a beam (NaN counts as that): their continuations come last, by (r, t).  The sum's terms are fp32: continuations of
+ *                    one beam, and of beams with the same logits, are in the order of their scores; two of other beams may change places when they are closer than 2^-17.
  *                    workspace: smh_beam_select_workspace_bytes(...) bytes, any contents, 8-byte aligned; calls that overlap need one each.
  * smh_beam_reorder   row g * W + i of each of up to 16 tensors takes the contents of row g * W + parents[g, i] (int32, cut to 0 .. W - 1), in place.  tensors, strides
  *                    (bytes between rows), bytes (of a row that move) and units are host arrays; units[k] > 0: only the first *upto (int32 on the device) entries of

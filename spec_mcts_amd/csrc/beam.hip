@@ -4,8 +4,10 @@
 // equal ones by (beam, token).  A first launch goes over each row once, a workgroup per slice of it: the slice's values stay in registers while its n largest, its maximum and its
 // sum of exponentials are found.  A second one has a workgroup per group: it adds the slices' sums up and picks the n best of all lists (one step a bit of the score,
 // ended when just n are left above).
-//   Order: within a row the fp16 values order exactly; between rows the scores are compared in 64 bits, with sums in 64 bits of fp32 terms, so that
-//   candidates keep their order unless they are closer than the terms' roundings (2^-24 each) leave the sums.
+//   Order: within a row, and between rows of the same logits, the fp16 values order exactly.  Between other rows the scores are compared in 64 bits, with sums in 64 bits of fp32
+//   terms exp(x - m), m the slice's largest value.  With d = m - x a term is off by 2^-23 of itself (the exponential) and d * 2.3 * 2^-24 (difference, product and log2(e)); the mean of d, weighted
+//   by the terms, is at most log(vocab) (an entropy is), so a sum is off by less than 2^-18 for up to 2^24 columns (usually 2^-22): candidates of two rows keep their order
+//   from 2^-17 apart.  A value's error depends on its slice's maximum: rows of the same values in another order are as close as that, and equal only where they are one slice.
 // Bound: 2 bytes a logit from HBM; short of that by the exponentials and their 64-bit sums (512 rows of 32016: 17 us for the first launch, of which HBM needs 6.6) and, for few rows, by
 // two launches (4 rows: 6.6 and 5.0 us).
 //
@@ -174,7 +176,7 @@ __device__ __forceinline__ BeamRow beam_row(const SelectParams &p, long row) {
             if (i0 + i < p.slices) s += si[i] * (mi[i] == m ? 1.0 : exp((double)mi[i] - (double)m));
     }
     if (!(score > -INFINITY) || ended) return BeamRow{(double)score, __builtin_nanf(""), ended};
-    // (36 bits of the sum: rows of the same values in another order are equal)
+    // (36 bits of the sum: the order in which one slice's terms were added shows in the last of 53, and here only where a sum is next to a step)
     return BeamRow{(double)score - log(__longlong_as_double((__double_as_longlong(s) + (1 << 15)) & ~0xFFFFll)), m, 0};
 }
 constexpr uint32_t BEAM_NONE = 0xFFFFFFFFu;        // (beam * vocab + token is below 2^30)

@@ -64,6 +64,40 @@ def test_sizes(G, W, n, vocab, ended):
     check(logits_of(G * W, vocab, vocab), scores, W, n, done, eos=min(EOS, vocab - 1))
 
 
+def rearranged(rows, vocab, seed):
+    """a row and the same values in other orders"""
+    g = torch.Generator().manual_seed(seed)
+    x = logits_of(1, vocab, seed)[0]
+    return torch.stack([x] + [x[torch.randperm(vocab, generator=g)] for _ in range(rows - 1)])
+
+
+@pytest.mark.parametrize("groups", [1, 80])
+@pytest.mark.parametrize("vocab", [8000, 32016, 129280])
+def test_beams_of_the_same_values_in_another_order(groups, vocab):
+    """their true scores are equal: apart by the least distance that keeps an order (2^-17) they are in it, by twice that"""
+    W = 7
+    x = rearranged(W, vocab, vocab).repeat(groups, 1)
+    check(x, (-torch.arange(W) * 2.0 ** -16).repeat(groups), W, 64)
+    check(x, (torch.arange(W) * 2.0 ** -16 - 1).repeat(groups), W, 64)
+
+
+@pytest.mark.parametrize("vocab", [3000, 8192, 32016])
+def test_equal_beams_of_the_same_values(vocab):
+    """at equal scores too the values are in their order, each beam's candidates in that of their tokens, and scores are as close as is said; beams of one slice are in order"""
+    W, n = 6, 60
+    x = rearranged(W, vocab, vocab + 1)
+    s, parents, tokens, _ = (t.cpu() for t in K().beam_select(x.to(DEV), torch.zeros(W, device=DEV), W, n))
+    value = x[parents[0].long(), tokens[0]].float()
+    assert bool((value.diff() <= 0).all())
+    exact = torch.log_softmax(x[:1].double(), 1)[0].max()
+    assert bool((s[0].double() - (exact + (value.double() - value[0].double()))).abs().max() <= 2.0 ** -18 + 2.0 ** -24 * 16)
+    for a, b in zip(range(n - 1), range(1, n)):
+        if value[a] == value[b] and (parents[0, a] == parents[0, b] or vocab <= 8192):
+            assert (parents[0, a], tokens[0, a]) < (parents[0, b], tokens[0, b])
+    top = x[0].float().sort(descending=True).values.repeat_interleave(W)[:n]
+    assert torch.equal(value, top)
+
+
 def test_more_rows_than_a_grid_has():
     check(logits_of(70000, 9, 3), -torch.rand(70000, generator=torch.Generator().manual_seed(3)), 1, 3)
     check(logits_of(70000, 9, 4), -torch.rand(70000, generator=torch.Generator().manual_seed(4)), 10, 12)
