@@ -55,17 +55,13 @@ __device__ __forceinline__ float max_of_groups(float v) {
     return fmaxf(r[0], r[1]);
 }
 
-// The largest power of two that is not above x (a scale: 2^-24 / 127 at least; below 2^-60, which none is, as if it were that), and 1 / that
-__device__ __forceinline__ float power_below(float x) { return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, fmaxf(x, 0x1p-60f)) & 0x7F800000u); }
-__device__ __forceinline__ float inverse_power(float p) { return __builtin_bit_cast(float, 0x7F000000u - __builtin_bit_cast(uint32_t, p)); }
-
 // A wave's queries: QT tiles of 16 columns, lane l has column l % 16.
 template <int QT>
 struct Kv8Wave {
     h8 q[QT][4];
     f4 o[QT][8];                                   // in units of `unit`
     float m[QT], l[QT];                            // the weights' reference, at most LAZY below the largest score; l: of the lane's own rows
-    float unit;                                    // a power of two, at most 2^FALL above and less than twice below the scale of V that the wave had last; 0: none yet
+    float unit;                                    // 1 .. 2^FALL times the scale of V that the wave had last; 0: none yet
     int at[QT];                                    // place of the query, -1: none
     int lo, hi;                                    // least and largest place of the wave's queries
 
@@ -90,26 +86,33 @@ struct Kv8Wave {
     }
 
     // Scores of 64 rows -> weights, as the second product takes them: p * f, f = v_scale / unit, with the factor in the exponent and taken out of l again, so that
-    // the product adds up in `unit`s by itself.  l must not lose a row because its V is small: the unit follows the scales both ways, so that f stays in 2^-FALL .. 2, and the sums
-    // go with it - by powers of two, which round nothing, however often blocks of large and of small values take turns.  (A block of zeros has no scale: its weights count in l alone.)
+    // the product adds up in `unit`s by itself.  l must not lose a row because its V is small, so f stays in 2^-FALL .. 1: the unit goes up to a larger scale, and down to a far smaller
+    // one by a power of two, and the sums go with it (exactly, where blocks of large and of small values take turns).  A block of zeros has no scale: its weights count in l alone.
     // masked: some row of the block may be out of some query's sight.  seen[t]: the lane's query sees a row of the block.
-    // The reference follows the largest score only when that is 2^LAZY of weight ahead, and stands for a weight of 2^RAISE: weights are below 2^15, and fp16's least exponent takes bits only
+    // The reference follows the largest score only when that is 2^LAZY of weight ahead, and stands for a weight of 2^RAISE: weights are at most 2^14, and fp16's least exponent takes bits only
     // from those below 2^-22 / f of the largest, which is 2^-20 at most.  l adds up the rounded weights, so that what the sums are divided by is what they were made with.
     static constexpr float LAZY = 6.0f, RAISE = 8.0f;
     static constexpr int FALL = 2;
     __device__ __forceinline__ void softmax(f4 (&x)[QT][4], float scale, float v_scale, int block, bool masked, int limit, int window, int sinks, h8 (&w)[QT][2], bool (&seen)[QT]) {
         const int g = (threadIdx.x & 63) >> 4;
-        // (by the exponents, FALL + 1 of which f may have: compared as numbers the bounds cost the reads 1 % of their rate)
+        // (compared as bits, which order as positive numbers do: as numbers the two bounds cost the reads 1 % of their rate)
         const uint32_t above = __builtin_bit_cast(uint32_t, v_scale) - (__builtin_bit_cast(uint32_t, unit) - ((uint32_t)FALL << 23));
-        if (above >= (uint32_t)(FALL + 1) << 23 && v_scale > 0.0f) {
-            const float now = power_below(v_scale), by = unit * inverse_power(now);
+        if (above > (uint32_t)FALL << 23 && v_scale > 0.0f) {
+            float now = v_scale;
+            if (v_scale < unit) {
+                now = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, unit) & 0x7FFFFFu) | (__builtin_bit_cast(uint32_t, v_scale) & 0x7F800000u));
+                if (now < v_scale) now *= 2.0f;
+            }
+            const float by = unit / now;
 #pragma unroll
             for (int t = 0; t < QT; ++t)
 #pragma unroll
                 for (int d = 0; d < 8; ++d) o[t][d] *= by;
             unit = now;
         }
-        const float f = v_scale == 0.0f ? 1.0f : v_scale * inverse_power(unit);      // (NaN stays NaN)
+        // v_scale / unit: Markstein's correction of the quotient by an approximate reciprocal with its remainder (NaN stays NaN)
+        const float inverse = __builtin_amdgcn_rcpf(unit), about = v_scale * inverse;
+        const float f = v_scale == 0.0f ? 1.0f : __builtin_fmaf(__builtin_fmaf(-about, unit, v_scale), inverse, about);
         const float log_f = __builtin_amdgcn_logf(f), inverse_f = __builtin_amdgcn_rcpf(f);
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
@@ -198,7 +201,7 @@ __device__ __forceinline__ void kv8_open_block(Kv8Wave<QT> &w, const Kv8AttnPara
     bool seen[QT];
     if (w.unit == 0.0f) w.unit = 1.0f;
     w.softmax(x, KV8_SCORE_SCALE, w.unit, block, true, block * KV8_ROWS + rows, p.window, p.sinks, pr, seen);
-    const float by = inverse_power(w.unit);        // (V's values are in units of 1)
+    const float by = 1.0f / w.unit;                // (V's values are in units of 1; a scale is 2^-24 / 127 at least)
 #pragma unroll
     for (int d = 0; d < 8; ++d) {
         h8 a[2];
