@@ -8,8 +8,8 @@
 //   terms exp(x - m), m the slice's largest value.  With d = m - x a term is off by 2^-23 of itself (the exponential) and d * 2.3 * 2^-24 (difference, product and log2(e)); the mean of d, weighted
 //   by the terms, is at most log(vocab) (an entropy is), so a sum is off by less than 2^-18 for up to 2^24 columns (usually 2^-22): candidates of two rows keep their order
 //   from 2^-17 apart.  A value's error depends on its slice's maximum: rows of the same values in another order are as close as that, and equal only where they are one slice.
-// Bound: 2 bytes a logit from HBM; short of that by the exponentials and their 64-bit sums (512 rows of 32016: 17 us for the first launch, of which HBM needs 6.6) and, for few rows, by
-// two launches (4 rows: 6.6 and 5.0 us).
+// Bound: 2 bytes a logit from HBM, and short of that because all workgroups of the first launch run at a time and go through loads, bar, candidates and exponentials together, so that the
+// phases add up (512 rows of 32016: 17 us, of which HBM needs 5.4; 1600 rows: 36, of which loads 17.5, bar 2, candidates 7, exponentials and sums 10); for few rows by two launches (4 rows: 6.5 and 4.9 us).
 //
 // Reordering.  Row i of a group takes the contents of row parents[i], in place: a workgroup owns a strip of all rows of a group, has it in LDS and then writes.
 // Bound: HBM, each row that another one takes read and each row that changes written once (64 rows of four layers' open blocks, 2 MB each, 17.5 us; 73 with four bytes a thread at a time).
@@ -449,7 +449,7 @@ extern "C" int smh_beam_select(const void *logits, long ld, const float *scores,
         else hipLaunchKernelGGL(beam_slice_kernel<4>, dim3(plan.slices, rows), dim3(256), n * 128, st, part);
         if (int rc = launch_status()) return rc;
     }
-    // (us a call of 32016 columns: 64 beams, 128 kept, 65, by the merge 253; 32 beams, 64 kept, 34 and 87)
+    // (us a call of 32016 columns: 64 beams, 128 kept, 65, by the merge 253; 32 beams, 64 kept, 34 and 87.  32 candidates a thread of 16 waves spill 26 vector registers)
     const long all = (long)W * plan.slices * n;
     if (all <= 256) hipLaunchKernelGGL((beam_pick_kernel<4, 1>), dim3(G), dim3(64), 0, st, p);
     else if (all <= 1024) hipLaunchKernelGGL((beam_pick_kernel<4, 4>), dim3(G), dim3(256), 0, st, p);

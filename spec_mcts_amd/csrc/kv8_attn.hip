@@ -225,7 +225,7 @@ __device__ __forceinline__ void kv8_open_block(Kv8Wave<QT> &w, const Kv8AttnPara
 // ---- up to 32 queries a sequence and kv head ------------------------------------------------------------------------------------
 // The four waves of a workgroup take alternate blocks of their part of the sequence, each for all queries (QT tiles), straight from memory into the operands: K of the
 // next block is asked for behind the products with this one's, V ahead of them.  Their states meet in LDS.
-// Bound by HBM: 80 sequences of up to 8192 rows, 64 heads over 8, 187 us (926 MB, 4.96 TB/s); 16 windows of 4096 rows of 32 heads 100 us (538 MB, 5.4 TB/s).
+// Bound by HBM: 80 sequences of up to 8192 rows, 64 heads over 8, 187 us (926 MB, 4.96 TB/s: uneven lengths, of one length 5.8 .. 6.05); 16 windows of 4096 rows of 32 heads 100 us (538 MB, 5.4 TB/s).
 // Two waves a SIMD: with three the registers do not suffice (us, two and three: 194 and 202, 108 and 117).
 template <int QT>
 __global__ __launch_bounds__(256, 2) void kv8_attn_few_kernel(Kv8AttnParams p) {
