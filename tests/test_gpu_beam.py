@@ -74,7 +74,7 @@ def rearranged(rows, vocab, seed):
 @pytest.mark.parametrize("groups", [1, 80])
 @pytest.mark.parametrize("vocab", [8000, 32016, 129280])
 def test_beams_of_the_same_values_in_another_order(groups, vocab):
-    """their true scores are equal: apart by the least distance that keeps an order (2^-17) they are in it, by twice that"""
+    """rows whose true sums are equal: with scores 2^-16 apart, twice the distance from which an order is kept, candidates are in it"""
     W = 7
     x = rearranged(W, vocab, vocab).repeat(groups, 1)
     check(x, (-torch.arange(W) * 2.0 ** -16).repeat(groups), W, 64)
